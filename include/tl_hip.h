@@ -275,6 +275,35 @@ tlhip_status tlhip_tensor_argmax(tlhip_ctx ctx, tlhip_tensor x, int dim, int kee
 tlhip_status tlhip_temperature_sample(tlhip_ctx ctx, tlhip_tensor logits, float temperature, uint64_t seed,
                                       uint64_t counter, int32_t* out);
 
+/* The softmax statistics of rows of logits ([V] or [rows, V], f16 or f32),
+ * beside softmax() and temperature_sample(); no counterpart in the
+ * reference.  For each row: logprob = log softmax(logits)[ids[row]] (ids I32
+ * [rows]; both or neither NULL), entropy (nats; may be NULL), and with n_top
+ * > 0 the n_top most likely tokens, top_ids I32 [rows, n_top] in falling
+ * order (ties: the lower index first) and their top_logprob.  logprob,
+ * entropy and top_logprob are F32.  -inf logits have probability 0 and their
+ * log probability is -inf.  A row with a NaN or +inf, or of -inf alone, has
+ * no distribution: NaN, and top_ids -1.  An id outside [0, V) gives NaN.
+ * n_top <= min(64, V).                                                     */
+tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tensor ids, int n_top,
+                                  tlhip_tensor logprob, tlhip_tensor entropy, tlhip_tensor top_logprob,
+                                  tlhip_tensor top_ids);
+
+/* A mixture-of-experts feed-forward layer for a few tokens, beside the dense
+ * one (linear, silu_mul, linear); no counterpart in the reference.
+ *   l = router x;  T = the top_k largest of l (ties: the first expert)
+ *   g = softmax(l) on T, divided by its sum over T if normalize
+ *   y = sum over e in T of g_e down_e (silu(gate_e x) * (up_e x))
+ * x and y [M, K], router [E, K], all f16; gate and up [E * I, K] and down
+ * [E * K, I], the experts' rows one after another (f16 also [E, I, K] and
+ * [E, K, I]), each F16, Q4_0 or Q8_0, gate and up of one type.  K and I are
+ * multiples of 32, E <= 256, top_k <= min(E, 32).  The weights count as the
+ * f16 values that linear() reads them as; what lies between x and y is not
+ * rounded to f16.  y may be x.  Any M; the weights an expert's tokens need
+ * are read once for up to 256 tokens.                                      */
+tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor router, tlhip_tensor gate, tlhip_tensor up,
+                       tlhip_tensor down, int top_k, int normalize, tlhip_tensor y);
+
 /* ---- KV cache (model::llama::Cache, llama.rs:50-114; KVCache builtins
  *      eval.rs:1247-1400), preallocated instead of concat-grown ----------- */
 typedef struct tlhip_kvcache_s* tlhip_kvcache;
@@ -291,6 +320,23 @@ tlhip_status tlhip_kvcache_create(tlhip_ctx ctx, int n_layers, int max_ctx, int 
  * points below are f16 (a DtypeError on an f32 cache).                    */
 tlhip_status tlhip_kvcache_create_f32(tlhip_ctx ctx, int n_layers, int max_ctx, int n_kv_heads,
                                       int head_dim, tlhip_kvcache* out);
+/* An 8-bit cache, about half an f16 one's memory; no counterpart in the
+ * reference.  Its set / append take f16 rows.  Blocks of 32 consecutive
+ * positions of one KV head, K and V apart, are kept as int8 with one f32
+ * scale: a = max |x|, q = round(x * (127 / a)), value q * (a / 127).  The
+ * rows past the last whole block (at most 31) are kept as they are until
+ * their block is whole, so what the cache holds depends on its rows and not
+ * on the calls that brought them.  get_k / get_v return a copy [len, Hkv, D]
+ * in f16 (later appends do not change it); the attention entry points read
+ * the int8 values with their scales, unrounded, and keep scores, weights and
+ * sums in f32 (the scale argument is not rounded to f16, and a position a
+ * query does not see weighs nothing).  K and V should be finite: a block
+ * (past the last whole one: a row) of a head that holds an infinity or NaN
+ * shows as NaN to the queries that see it.  head_dim 32, 64, 80, 96, 128 or
+ * 256, at most 1024 KV heads; used on the context it was created on only
+ * (else InvalidArgument).                                                  */
+tlhip_status tlhip_kvcache_create_q8(tlhip_ctx ctx, int n_layers, int max_ctx, int n_kv_heads,
+                                     int head_dim, tlhip_kvcache* out);
 tlhip_status tlhip_kvcache_free(tlhip_kvcache c);
 /* cache.set(layer, K, V): replaces the layer's contents with K,V [S,Hkv,D]
  * (K and V of the same shape, else ShapeMismatch).                       */

@@ -139,6 +139,21 @@ void ctx_release(tlhip_ctx ctx);
 tlhip_status check_t(tlhip_tensor t, const char* what);
 tlhip_status check_dtype(tlhip_tensor t, tlhip_dtype d, const char* op);
 tlhip_status after_launch(tlhip_ctx ctx, const char* op);
+// A tensor of ctx's device (another device's is refused).
+tlhip_status check_here(tlhip_ctx ctx, tlhip_tensor t, const char* op);
+// Makes a device current for a call and puts the caller's back.
+struct DeviceScope {
+    int prev = -1;
+    explicit DeviceScope(int device) {
+        int cur = device;
+        if (hipGetDevice(&cur) == hipSuccess && cur != device && hipSetDevice(device) == hipSuccess) prev = cur;
+    }
+    ~DeviceScope() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
 
 // Internal allocation of a tensor (used by ops, model and kvcache code).
 tlhip_status alloc_tensor(tlhip_ctx ctx, tlhip_dtype dtype, int ndim, const int64_t* shape,
@@ -389,8 +404,103 @@ tlhip_status launch_attention_mfma(hipStream_t s, const AttnArgs& a, int J, uint
 constexpr int kAttnRowKeys = 8192;    // keys the one-workgroup kernels hold in their LDS score row
 constexpr int kAttnMaxKeys = 65536;   // keys any attention entry point reads (longer rows take the
                                       // key-chunked split for one query row, the matrix cores for more)
+// The 8-bit KV cache (kernels_kv8.hip has the layout).
+struct Kv8Layer {
+    tlhip_tensor buf = nullptr;   // one allocation, cut into the following
+    uint8_t *kq = nullptr, *vq = nullptr;          // tiles [n_kv][n_blocks][32 * D]
+    float *ks = nullptr, *vs = nullptr;            // scales [n_kv][n_blocks]
+    uint16_t *tail_k = nullptr, *tail_v = nullptr; // f16 tiles [2][n_kv][32 * D]
+    float* tail_flag = nullptr;                    // [2][n_kv][32]: 0, NaN for a non-finite row of V
+    int tail_cur = 0;                              // which of the two tails is the layer's
+};
+struct Kv8Write {
+    const uint16_t *k = nullptr, *v = nullptr;     // [S, n_kv, D]
+    uint8_t *kq = nullptr, *vq = nullptr;
+    float *ks = nullptr, *vs = nullptr;
+    uint16_t *tail_k = nullptr, *tail_v = nullptr;
+    float* tail_flag = nullptr;
+    int tail_src = 0, tail_dst = 0;
+    int len0 = 0, S = 0, n_full = 0;               // positions before, new rows, blocks they complete
+    int n_kv = 0, D = 0, n_blocks = 0;
+};
+struct Kv8Read {
+    const uint8_t* q = nullptr;
+    const float* s = nullptr;
+    const uint16_t* tail = nullptr;
+    const float* tail_flag = nullptr;
+    uint16_t* out = nullptr;                       // [len, n_kv, D]
+    int tail_cur = 0, len = 0, n_kv = 0, D = 0, n_blocks = 0, is_v = 0;
+};
+struct Kv8Attn {
+    const uint16_t* q = nullptr;                   // [S, H, D]
+    uint16_t* out = nullptr;
+    const uint8_t *kq = nullptr, *vq = nullptr;
+    const float *ks = nullptr, *vs = nullptr;
+    const uint16_t *tail_k = nullptr, *tail_v = nullptr;
+    const float* tail_flag = nullptr;
+    float* scratch = nullptr;
+    float scale = 1.0f;
+    int tail_cur = 0, n_full = 0;                  // whole blocks
+    int S = 0, H = 0, n_kv = 0, group = 0, D = 0, n_blocks = 0, q_pos0 = 0, splits = 1;
+};
+struct Kv8Plan {
+    int nq = 1;                // 16-row columns of a wave
+    int splits = 0;            // key splits (0: a wave walks all keys of its rows)
+    size_t scratch_bytes = 0;
+};
+bool kv8_head_dim_ok(int D);
+Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len);
+tlhip_status launch_kv8_write(hipStream_t s, const Kv8Write& p);
+tlhip_status launch_kv8_read(hipStream_t s, const Kv8Read& p);
+tlhip_status launch_kv8_attention(hipStream_t s, const Kv8Attn& p, const Kv8Plan& pl);
+
+// log-softmax statistics of rows of logits (kernels_logprobs.hip)
+struct LogprobArgs {
+    const void* x = nullptr;          // [rows, V], f16 or f32
+    const int32_t* ids = nullptr;     // [rows] or none
+    float *logprob = nullptr, *entropy = nullptr, *top_logprob = nullptr;
+    int32_t* top_ids = nullptr;
+    int rows = 0, V = 0, n_top = 0;
+    bool f32 = false;
+};
+constexpr int kMaxTop = 64;           // alternatives of token_logprobs
+tlhip_status launch_logprobs(hipStream_t s, const LogprobArgs& a);
+
+// mixture-of-experts layer (kernels_moe.hip)
+struct MoeArgs {
+    const uint16_t *x = nullptr, *router = nullptr;   // [M, K], [E, K]
+    const void *gate = nullptr, *up = nullptr, *down = nullptr;   // [E * I, K] twice, [E * K, I]
+    const uint16_t *gate_d = nullptr, *up_d = nullptr, *down_d = nullptr;
+    uint16_t* y = nullptr;            // [M, K]
+    int32_t* ids = nullptr;           // workspace: [M, top] chosen experts
+    float* g = nullptr;               // [M, top] their weights
+    float* h = nullptr;               // [M * top, I]
+    int M = 0, K = 0, I = 0, E = 0, top = 0, normalize = 0;
+    int wt_gu = 0, wt_down = 0;
+};
+constexpr int kMoeMaxExperts = 256, kMoeMaxTop = 32;
+tlhip_status launch_moe(hipStream_t s, const MoeArgs& a);
+
 tlhip_status launch_copy_rows(hipStream_t s, const uint16_t* src, uint16_t* dst, int rows,
                               int row_elems, int src_stride, int dst_stride, const int32_t* d_pos,
                               int dst_row0);
 
+}  // namespace tlhip
+
+struct tlhip_kvcache_s {
+    tlhip_ctx ctx = nullptr;
+    tlhip_dtype dtype = TLHIP_F16;   // KVCache::new_f16 / new_f32; TLHIP_Q8_0: the 8-bit cache
+    int n_layers = 0, max_ctx = 0, n_kv = 0, head_dim = 0;
+    std::vector<tlhip_tensor> k, v;  // f16 / f32
+    std::vector<tlhip::Kv8Layer> q8;
+    std::vector<int> len;
+};
+
+namespace tlhip {
+// the 8-bit cache behind tlhip_kvcache_* and the attention entry points (kv8.cpp)
+tlhip_status kv8_alloc(tlhip_kvcache c);
+// (kv8_write: rows of checked shape at positions start .. start + S - 1, the layer's end or 0)
+tlhip_status kv8_write(tlhip_ctx ctx, tlhip_kvcache c, int layer, tlhip_tensor k, tlhip_tensor v, int start, int S);
+tlhip_status kv8_get(tlhip_kvcache c, int layer, int which_v, tlhip_tensor* out);
+tlhip_status kv8_attention(tlhip_ctx ctx, tlhip_tensor q, tlhip_kvcache c, int layer, float scale, tlhip_tensor out);
 }  // namespace tlhip

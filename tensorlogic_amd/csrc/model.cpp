@@ -31,14 +31,6 @@
 
 using namespace tlhip;
 
-struct tlhip_kvcache_s {
-    tlhip_ctx ctx = nullptr;
-    tlhip_dtype dtype = TLHIP_F16;   // KVCache::new_f16 / new_f32
-    int n_layers = 0, max_ctx = 0, n_kv = 0, head_dim = 0;
-    std::vector<tlhip_tensor> k, v;
-    std::vector<int> len;
-};
-
 namespace {
 
 struct Lin {
@@ -671,6 +663,15 @@ static tlhip_status kvcache_create(tlhip_ctx ctx, int n_layers, int max_ctx, int
     c->n_kv = n_kv_heads;
     c->head_dim = head_dim;
     c->len.assign(n_layers, 0);
+    if (dtype == TLHIP_Q8_0) {
+        const tlhip_status st = kv8_alloc(c);
+        if (st != TLHIP_OK) {
+            tlhip_kvcache_free(c);
+            return st;
+        }
+        *out = c;
+        return TLHIP_OK;
+    }
     int64_t shp[3] = {max_ctx, n_kv_heads, head_dim};
     for (int i = 0; i < n_layers; i++) {
         tlhip_tensor k = nullptr, v = nullptr;
@@ -698,8 +699,14 @@ tlhip_status tlhip_kvcache_create_f32(tlhip_ctx ctx, int n_layers, int max_ctx, 
     return kvcache_create(ctx, n_layers, max_ctx, n_kv_heads, head_dim, TLHIP_F32, out);
 } TLHIP_CATCH_STATUS
 
+tlhip_status tlhip_kvcache_create_q8(tlhip_ctx ctx, int n_layers, int max_ctx, int n_kv_heads, int head_dim,
+                                     tlhip_kvcache* out) try {
+    return kvcache_create(ctx, n_layers, max_ctx, n_kv_heads, head_dim, TLHIP_Q8_0, out);
+} TLHIP_CATCH_STATUS
+
 tlhip_status tlhip_kvcache_free(tlhip_kvcache c) try {
     if (!c) return TLHIP_OK;
+    for (auto& l : c->q8) tlhip_tensor_free(l.buf);
     for (auto t : c->k) tlhip_tensor_free(t);
     for (auto t : c->v) tlhip_tensor_free(t);
     delete c;
@@ -711,8 +718,9 @@ static tlhip_status kv_write(tlhip_ctx ctx, tlhip_kvcache c, int layer, tlhip_te
     if (!c || layer < 0 || layer >= c->n_layers) return fail(TLHIP_ERR_INDEX_OUT_OF_BOUNDS, "kvcache layer %d", layer);
     TLHIP_TRY(check_t(k, "kvcache K"));
     TLHIP_TRY(check_t(v, "kvcache V"));
-    TLHIP_TRY(check_dtype(k, c->dtype, "kvcache"));
-    TLHIP_TRY(check_dtype(v, c->dtype, "kvcache"));
+    const tlhip_dtype rows = c->dtype == TLHIP_Q8_0 ? TLHIP_F16 : c->dtype;
+    TLHIP_TRY(check_dtype(k, rows, "kvcache"));
+    TLHIP_TRY(check_dtype(v, rows, "kvcache"));
     const int64_t row = (int64_t)c->n_kv * c->head_dim;
     // K and V must have the same shape: same element count alone would let a
     // V of another layout (e.g. [S, D, Hkv]) be stored as if it were [S, Hkv, D]
@@ -724,6 +732,11 @@ static tlhip_status kv_write(tlhip_ctx ctx, tlhip_kvcache c, int layer, tlhip_te
     const int start = append ? c->len[layer] : 0;
     if (start + S > c->max_ctx)
         return fail(TLHIP_ERR_INDEX_OUT_OF_BOUNDS, "kvcache: %d + %d rows > %d", start, S, c->max_ctx);
+    if (c->dtype == TLHIP_Q8_0) {
+        TLHIP_TRY(kv8_write(ctx, c, layer, k, v, start, S));
+        c->len[layer] = start + S;
+        return TLHIP_OK;
+    }
     // (rows copied as 16-bit units: an f32 row is twice as many)
     const int ru = (int)row * (c->dtype == TLHIP_F32 ? 2 : 1);
     TLHIP_TRY(launch_copy_rows(ctx->stream, P(k), P(c->k[layer]), S, ru, ru, ru, nullptr, start));
@@ -744,6 +757,7 @@ tlhip_status tlhip_kvcache_get(tlhip_kvcache c, int layer, int which_v, tlhip_te
     if (!c || !out || layer < 0 || layer >= c->n_layers)
         return fail(TLHIP_ERR_INDEX_OUT_OF_BOUNDS, "kvcache layer %d", layer);
     if (c->len[layer] == 0) return fail(TLHIP_ERR_INVALID_OPERATION, "kvcache layer %d is empty", layer);
+    if (c->dtype == TLHIP_Q8_0) return kv8_get(c, layer, which_v, out);
     tlhip_tensor src = which_v ? c->v[layer] : c->k[layer];
     int64_t shp[3] = {c->len[layer], c->n_kv, c->head_dim};
     // a view of the first len rows: same storage, shorter leading dim
@@ -775,6 +789,7 @@ tlhip_status tlhip_attention_prefill(tlhip_ctx ctx, tlhip_tensor q, tlhip_kvcach
     const int64_t S = q->shape[0];
     if (S < 1 || S > len)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "attention: %lld query rows for a cache of %d rows", (long long)S, len);
+    if (c->dtype == TLHIP_Q8_0) return kv8_attention(ctx, q, c, layer, scale, out);
     tlhip_tensor k = nullptr, v = nullptr;
     TLHIP_TRY(tlhip_kvcache_get(c, layer, 0, &k));
     tlhip_status st = tlhip_kvcache_get(c, layer, 1, &v);

@@ -131,6 +131,13 @@ tlhip_status check_dtype(tlhip_tensor t, tlhip_dtype d, const char* op) {
     return TLHIP_OK;
 }
 
+tlhip_status check_here(tlhip_ctx ctx, tlhip_tensor t, const char* op) {
+    if (t->ctx->device != ctx->device)
+        return fail(TLHIP_ERR_INVALID_ARGUMENT, "%s: a tensor of device %d on a context of device %d", op,
+                    t->ctx->device, ctx->device);
+    return TLHIP_OK;
+}
+
 tlhip_status after_launch(tlhip_ctx ctx, const char* op) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(TLHIP_ERR_DEVICE, "%s launch failed: %s", op, hipGetErrorString(e));

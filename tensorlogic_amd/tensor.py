@@ -358,15 +358,46 @@ def temperature_sample(logits: Tensor, temperature: float, seed: int = 0, counte
     return out.value
 
 
+def token_logprobs(logits: Tensor, ids: Tensor | None = None, n_top: int = 0):
+    """What the softmax of each row of logits ([V] or [rows, V], f16 or f32)
+    says: (logprob, entropy, top_logprob, top_ids).  logprob [rows] is that of
+    the tokens ids (I32 [rows]; None without ids), entropy [rows] in nats, and
+    top_logprob / top_ids [rows, n_top] the likeliest tokens in falling order
+    (None for n_top = 0).  F32 and I32 tensors; nothing waits."""
+    dev, shape = logits.dev, logits.shape
+    rows = shape[0] if len(shape) == 2 else 1
+    logprob = dev.empty((rows,), F32) if ids is not None else None
+    entropy = dev.empty((rows,), F32)
+    top = n_top > 0   # (a negative n_top: the library refuses it)
+    top_logprob, top_ids = (dev.empty((rows, n_top), F32), dev.empty((rows, n_top), I32)) if top else (None, None)
+    call("tlhip_token_logprobs", dev.h, logits.h, ids.h if ids is not None else None, int(n_top),
+         logprob.h if logprob is not None else None, entropy.h, top_logprob.h if top else None,
+         top_ids.h if top else None)
+    return logprob, entropy, top_logprob, top_ids
+
+
+def moe(x: Tensor, router: Tensor, gate: Tensor, up: Tensor, down: Tensor, top_k: int, normalize: bool = True) -> Tensor:
+    """A mixture-of-experts feed-forward layer of a few tokens x [M, K]: the
+    top_k experts of router [E, K] (softmax weights, over their sum if
+    normalize), each down(silu(gate x) * up x), summed.  gate, up [E * I, K]
+    and down [E * K, I] hold the experts' rows one after another (F16, Q4_0
+    or Q8_0)."""
+    out = x.dev.empty(x.shape)
+    call("tlhip_moe", x.dev.h, x.h, router.h, gate.h, up.h, down.h, int(top_k), int(bool(normalize)), out.h)
+    return out
+
+
 class KVCache:
     """KVCache::new_f16 (or, dtype F32, KVCache::new_f32) with a
-    preallocated device buffer per layer."""
+    preallocated device buffer per layer; dtype Q8_0: the 8-bit cache (f16
+    rows in, blocks of 32 positions of a head quantised with one scale, get_k
+    / get_v copies in f16)."""
 
     def __init__(self, dev: Device, n_layers: int, max_ctx: int, n_kv_heads: int, head_dim: int,
                  dtype: int = F16):
         self.dev = dev
         h = _vp()
-        fn = "tlhip_kvcache_create_f32" if dtype == F32 else "tlhip_kvcache_create"
+        fn = {F32: "tlhip_kvcache_create_f32", Q8_0: "tlhip_kvcache_create_q8"}.get(dtype, "tlhip_kvcache_create")
         call(fn, dev.h, n_layers, max_ctx, n_kv_heads, head_dim, C.byref(h))
         self.h = h
 
