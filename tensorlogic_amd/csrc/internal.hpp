@@ -460,10 +460,18 @@ struct LogprobArgs {
     const int32_t* ids = nullptr;     // [rows] or none
     float *logprob = nullptr, *entropy = nullptr, *top_logprob = nullptr;
     int32_t* top_ids = nullptr;
+    float* part = nullptr;            // [rows, chunks, 4] sums of each chunk
+    uint64_t* part_keys = nullptr;    // [rows, chunks, n_top]
     int rows = 0, V = 0, n_top = 0;
+    int chunks = 1, chunk = 0;        // workgroups of a row, elements of each
     bool f32 = false;
 };
 constexpr int kMaxTop = 64;           // alternatives of token_logprobs
+struct LogprobPlan {
+    int chunks = 1, chunk = 0;
+    size_t part_bytes = 0, ws_bytes = 0;   // workspace: part, then part_keys
+};
+LogprobPlan logprobs_plan(int rows, int V, int n_top);
 tlhip_status launch_logprobs(hipStream_t s, const LogprobArgs& a);
 
 // mixture-of-experts layer (kernels_moe.hip)

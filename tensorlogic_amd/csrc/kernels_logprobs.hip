@@ -3,8 +3,21 @@
 //
 // With m = max x, z = sum e^(x - m) and t = sum (x - m) e^(x - m):
 //   log p_i = (x_i - m) - log z,   H = log z - t / z.
-// One pass keeps m, z and t up to date: when m rises by -d, z becomes z e^d
-// and t becomes (t + d z) e^d.  All in f32.
+// One pass over the row keeps m, z and t up to date: when m rises by -d, z
+// becomes z e^d and t becomes (t + d z) e^d.  All in f32, in powers of two
+// (t in units of ln 2).
+//
+// The n largest come out of the same pass.  They are the n largest keys
+// (value up, index down), all different.  A workgroup's threads are 64 groups
+// of four; the n-th largest of the groups' largest keys so far is a bound tau
+// that n keys of the row are known to reach, so only keys from tau up are
+// kept: a thread compares its batch's maximum, which the softmax needs
+// anyway, and looks at single values only if that reaches tau.  tau is found
+// after the batches 1, 2, 4, 8, ...; on random rows a doubling adds about n
+// to 5 n keys to the list.  Rows made to defeat the bound (rising ones of
+// great length) overflow the list and are ranked by n rounds over the row.
+//
+// Few rows are cut into chunks, a workgroup each, joined by a second kernel.
 #include <cmath>
 
 #include "device_common.hpp"
@@ -15,32 +28,60 @@ namespace tlhip {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
+constexpr int kBatch = 8192;      // elements of a workgroup's batch: 32 per thread
+constexpr int kList = 2048, kRanked = 512;
+constexpr int kMaxChunks = 32;
 
+// The sums in reference to r: e = 2^d2(x).  f32: r = m and d2 = (x - m)
+// log2(e), which reaches the type's lowest value; f16: r = m log2(e) and d2 =
+// x log2(e) - r in one fused operation.  (Any r near the maximum will do, so
+// r's own rounding costs nothing.)
+template <bool F32>
 struct Stat {
-    float m, z, t;
-    static __device__ __forceinline__ Stat none() { return Stat{-3.4028234663852886e38f, 0.0f, 0.0f}; }
-    __device__ __forceinline__ void raise(float mn) {
-        const float d = m - mn, f = __builtin_amdgcn_exp2f(d * kLog2e);
+    float m, r, z, t;
+    static __device__ __forceinline__ Stat none() {
+        Stat s;
+        s.m = F32 ? -3.4028234663852886e38f : -65536.0f;   // below every finite logit, or the lowest
+        s.r = F32 ? s.m : s.m * kLog2e;
+        s.z = s.t = 0.0f;
+        return s;
+    }
+    __device__ __forceinline__ float d2(float x) const { return F32 ? (x - r) * kLog2e : __builtin_fmaf(x, kLog2e, -r); }
+    __device__ __forceinline__ void rise(float mn, float rn) {
+        const float d = F32 ? (r - rn) * kLog2e : r - rn, f = __builtin_amdgcn_exp2f(d);
         t = f > 0.0f ? fmaf(d, z, t) * f : 0.0f;   // (d may be infinite where f is 0)
         z *= f;
         m = mn;
+        r = rn;
     }
+    __device__ __forceinline__ void rise(float mn) { rise(mn, F32 ? mn : mn * kLog2e); }
     __device__ __forceinline__ void add(float x) {
-        if (x > m) raise(x);
-        const float d = x - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-        z += e;
-        t += e > 0.0f ? d * e : 0.0f;              // (-inf: nothing)
+        const float d = d2(x), e = __builtin_amdgcn_exp2f(d);
+        z += e;                                    // (a NaN or +inf shows in z)
+        t = fmaf(fmaxf(d, -300.0f), e, t);         // (-inf: -300 * 0)
     }
     __device__ __forceinline__ void join(Stat o) {
-        const float mn = fmaxf(m, o.m);
-        raise(mn);
-        o.raise(mn);
+        if (o.m > m) rise(o.m, o.r);
+        else o.rise(m, r);
         z += o.z;
         t += o.t;
     }
+    // a NaN or +inf among the logits, or nothing but -inf: no distribution
+    __device__ __forceinline__ bool ok() const { return z > 0.0f && z < INFINITY; }
+    __device__ __forceinline__ float logprob(float x, float lz2) const {
+        return F32 ? x - r - lz2 * kLn2 : (d2(x) - lz2) * kLn2;
+    }
+    __device__ __forceinline__ Stat from_lane(int mask) const {
+        Stat o;
+        o.m = __shfl_xor(m, mask, 64);
+        o.r = __shfl_xor(r, mask, 64);
+        o.z = __shfl_xor(z, mask, 64);
+        o.t = __shfl_xor(t, mask, 64);
+        return o;
+    }
 };
 
-// Keys ordered as the pairs (value up, index down); -0 is 0.
+// Keys ordered as the pairs (value up, index down); -0 is 0.  0: no key.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
@@ -49,70 +90,269 @@ __device__ __forceinline__ float key_value(uint64_t k) {
     const uint32_t b = (uint32_t)(k >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
 }
+__device__ __forceinline__ int32_t key_index(uint64_t k) { return (int32_t)(0xFFFFFFFFu - (uint32_t)k); }
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 template <bool F32>
-__device__ __forceinline__ float at(const LogprobArgs& a, int64_t i) {
+__device__ __forceinline__ float at(const LogprobArgs& a, size_t i) {
     return F32 ? ((const float*)a.x)[i] : h2f(((const uint16_t*)a.x)[i]);
 }
 
+// 32 elements of a thread, in vectors of 16 bytes a workgroup's width apart.
+struct __attribute__((packed, aligned(4))) f4_any {
+    float f[4];
+};
 template <bool F32>
-__global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
-    __shared__ Stat st[4];
-    __shared__ uint64_t best[4];
-    const int64_t row = blockIdx.x, base = row * a.V;
-    const int tid = threadIdx.x, wave = tid >> 6;
-    Stat s = Stat::none();
-    for (int i = tid; i < a.V; i += 256) s.add(at<F32>(a, base + i));
-    for (int k = 32; k; k >>= 1) {
-        Stat o;
-        o.m = __shfl_xor(s.m, k, 64);
-        o.z = __shfl_xor(s.z, k, 64);
-        o.t = __shfl_xor(s.t, k, 64);
-        s.join(o);
+struct Batch {
+    static constexpr int W = F32 ? 4 : 8, NV = 32 / W;
+    float f[F32 ? 32 : 1];
+    h8 h[F32 ? 1 : 4];
+    static __device__ __forceinline__ int index(int j) { return (j / W * 256 + (int)threadIdx.x) * W + j % W; }
+    __device__ __forceinline__ float operator[](int j) const {
+        if constexpr (F32) return f[j];
+        else return (float)h[j / 8][j % 8];
     }
-    if ((tid & 63) == 0) st[wave] = s;
-    __syncthreads();
-    s = st[0];
-    for (int k = 1; k < 4; k++) s.join(st[k]);
-    // a NaN or +inf among the logits, or nothing but -inf: no distribution
-    const bool ok = s.z > 0.0f && s.z < INFINITY;
-    const float lz = __builtin_amdgcn_logf(s.z) * kLn2;
-    if (tid == 0) {
-        if (a.logprob) {
-            const int id = a.ids[row];
-            a.logprob[row] = ok && id >= 0 && id < a.V ? at<F32>(a, base + id) - s.m - lz : NAN;
-        }
-        if (a.entropy) a.entropy[row] = ok ? lz - s.t / s.z : NAN;
-    }
-    uint64_t below = ~0ull;
-    for (int n = 0; n < a.n_top; n++) {
-        uint64_t b = 0;
-        if (ok)
-            for (int i = tid; i < a.V; i += 256) {
-                const uint64_t k = key_of(at<F32>(a, base + i), i);
-                if (k < below && k > b) b = k;
+    // elements base + index(j); -inf past `have` elements
+    __device__ __forceinline__ void load(const LogprobArgs& a, size_t base, int have) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int i = (v * 256 + (int)threadIdx.x) * W;
+            if constexpr (F32) {
+                const float* p = (const float*)a.x + base + i;
+                if (i + W <= have) {
+                    const f4_any w = *(const f4_any*)p;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[4 * v + e] = w.f[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[4 * v + e] = i + e < have ? p[e] : -INFINITY;
+                }
+            } else {
+                const uint16_t* p = (const uint16_t*)a.x + base + i;
+                if (i + W <= have) {
+                    const h8_any w = *(const h8_any*)p;
+                    h[v] = __builtin_bit_cast(h8, u4{w.w[0], w.w[1], w.w[2], w.w[3]});
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) h[v][e] = i + e < have ? __builtin_bit_cast(h16, p[e]) : (h16)-INFINITY;
+                }
             }
-        for (int k = 32; k; k >>= 1) {
-            const uint64_t o = __shfl_xor((unsigned long long)b, k, 64);
-            b = o > b ? o : b;
         }
-        __syncthreads();
-        if ((tid & 63) == 0) best[wave] = b;
-        __syncthreads();
-        for (int k = 0; k < 4; k++) b = best[k] > b ? best[k] : b;
-        if (tid == 0) {
-            a.top_logprob[row * a.n_top + n] = ok ? key_value(b) - s.m - lz : NAN;
-            a.top_ids[row * a.n_top + n] = ok ? (int32_t)(0xFFFFFFFFu - (uint32_t)b) : -1;
+    }
+};
+
+struct TopShared {
+    uint64_t group[64];
+    uint64_t list[kList], ranked[kRanked];
+    uint64_t best[4];
+    int count, kept;
+};
+
+// The n-th largest of the 64 groups' keys (0 if there are fewer), the same in
+// every thread.
+__device__ __forceinline__ uint64_t bound(uint64_t mine, int n, TopShared& sh) {
+    for (int k = 1; k < 4; k <<= 1) mine = max64(mine, __shfl_xor((unsigned long long)mine, k, 64));
+    __syncthreads();
+    if ((threadIdx.x & 3) == 0) sh.group[threadIdx.x >> 2] = mine;
+    __syncthreads();
+    const uint64_t g = sh.group[threadIdx.x & 63];
+    int above = 0;
+#pragma unroll 8
+    for (int k = 0; k < 64; k++) {
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)g, k), hi = __builtin_amdgcn_readlane((int)(g >> 32), k);
+        above += ((uint64_t)hi << 32 | lo) > g;
+    }
+    const uint64_t who = __ballot(above == n - 1 && g != 0);
+    if (!who) return 0;
+    const int src = __builtin_ctzll(who);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)g, src), hi = __builtin_amdgcn_readlane((int)(g >> 32), src);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// Writes the n largest of `count` keys in LDS to out in falling order, by
+// counting for each the keys above it.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int n, uint64_t* out) {
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const uint64_t k = keys[i];
+        int above = 0;
+        for (int j = 0; j < count; j++) above += keys[j] > k;
+        if (k && above < n) out[above] = k;
+    }
+}
+
+// The same by n rounds of the largest key below the last one; key(i), i <
+// count, may be read n times.
+template <typename KEY>
+__device__ __forceinline__ void rounds(const KEY& key, int count, int n, uint64_t* out, TopShared& sh) {
+    uint64_t below = ~0ull;
+    for (int r = 0; r < n; r++) {
+        uint64_t b = 0;
+        for (int i = threadIdx.x; i < count; i += 256) {
+            const uint64_t k = key(i);
+            if (k < below && k > b) b = k;
         }
+        for (int k = 32; k; k >>= 1) b = max64(b, __shfl_xor((unsigned long long)b, k, 64));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = b;
+        __syncthreads();
+        for (int k = 0; k < 4; k++) b = max64(b, sh.best[k]);
+        if (threadIdx.x == 0) out[r] = b;
         below = b;
     }
 }
 
+template <bool F32>
+__device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Stat<F32>& s, const uint64_t* top) {
+    const bool ok = s.ok();
+    const float lz2 = __builtin_amdgcn_logf(s.z);
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        if (a.logprob) {
+            const int id = a.ids[row];
+            a.logprob[row] = ok && id >= 0 && id < a.V ? s.logprob(at<F32>(a, (size_t)row * a.V + id), lz2) : NAN;
+        }
+        if (a.entropy) a.entropy[row] = ok ? (lz2 - s.t / s.z) * kLn2 : NAN;
+    }
+    if (tid < a.n_top) {
+        const uint64_t k = top[tid];
+        a.top_logprob[(size_t)row * a.n_top + tid] = ok ? s.logprob(key_value(k), lz2) : NAN;
+        a.top_ids[(size_t)row * a.n_top + tid] = ok ? key_index(k) : -1;
+    }
+}
+
+template <bool F32, bool TOP>
+__global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
+    __shared__ Stat<F32> st[4];
+    __shared__ __align__(16) uint8_t top_raw[TOP ? sizeof(TopShared) : 16];
+    __shared__ uint64_t top[TOP ? kMaxTop : 1];
+    TopShared& sh = *(TopShared*)top_raw;
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
+    const int begin = chunk * a.chunk, count = a.V - begin < a.chunk ? a.V - begin : a.chunk;
+    const size_t base = (size_t)row * a.V + begin;
+    Stat<F32> s = Stat<F32>::none();
+    uint64_t best = 0, tau = 0;
+    if (TOP) {
+        if (tid < kMaxTop) top[tid] = 0;
+        if (tid == 0) sh.count = sh.kept = 0;
+    }
+    for (int b = 0, nb = 0; b < count; b += kBatch, nb++) {
+        const int have = count - b;
+        Batch<F32> x;
+        x.load(a, base + b, have);
+        float m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 32; j++) m = fmaxf(m, x[j]);
+        if (m > s.m) s.rise(m);
+#pragma unroll
+        for (int j = 0; j < 32; j++) s.add(x[j]);
+        if constexpr (TOP) {
+            if (Batch<F32>::index(0) < have && (!best || m > key_value(best))) {
+                int first = 0;
+#pragma unroll
+                for (int j = 31; j >= 0; j--) first = x[j] == m && Batch<F32>::index(j) < have ? Batch<F32>::index(j) : first;
+                best = key_of(m, begin + b + first);
+            }
+            if (nb == 0) tau = bound(best, a.n_top, sh);
+            if (m >= key_value(tau) || !tau) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const int i = Batch<F32>::index(j);
+                    const uint64_t k = key_of(x[j], begin + b + i);
+                    if (i < have && k >= tau) {
+                        const int slot = atomicAdd(&sh.count, 1);
+                        if (slot < kList) sh.list[slot] = k;
+                    }
+                }
+            }
+            if (nb && !(nb & (nb + 1)) && b + kBatch < count) tau = bound(best, a.n_top, sh);
+        }
+    }
+    for (int k = 32; k; k >>= 1) s.join(s.from_lane(k));
+    if ((tid & 63) == 0) st[tid >> 6] = s;
+    __syncthreads();
+    s = st[0];
+    for (int k = 1; k < 4; k++) s.join(st[k]);
+    if constexpr (TOP) {
+        tau = bound(best, a.n_top, sh);
+        const int listed = sh.count;
+        if (listed <= kList) {
+            for (int i = tid; i < listed; i += 256) {
+                const uint64_t k = sh.list[i];
+                if (k >= tau) {
+                    const int slot = atomicAdd(&sh.kept, 1);
+                    if (slot < kRanked) sh.ranked[slot] = k;
+                }
+            }
+            __syncthreads();
+            const int kept = sh.kept;
+            if (kept <= kRanked) rank_keys(sh.ranked, kept, a.n_top, top);
+            else rounds([&](int i) { return sh.list[i]; }, listed, a.n_top, top, sh);
+        } else {
+            rounds([&](int i) { return key_of(at<F32>(a, base + i), begin + i); }, count, a.n_top, top, sh);
+        }
+        __syncthreads();
+    }
+    if (a.chunks == 1) {
+        finish<F32>(a, row, s, top);
+        return;
+    }
+    // the chunk's sums and keys, for logprobs_join_kernel
+    if (tid == 0) *(f4*)(a.part + 4 * (size_t)blockIdx.x) = f4{s.m, s.r, s.z, s.t};
+    if (TOP && tid < a.n_top) a.part_keys[(size_t)blockIdx.x * a.n_top + tid] = top[tid];
+}
+
+template <bool F32>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t keys[kMaxChunks * kMaxTop], top[kMaxTop];
+    const int row = blockIdx.x, n = a.chunks * a.n_top;
+    for (int i = threadIdx.x; i < n; i += 256) keys[i] = a.part_keys[(size_t)row * n + i];
+    Stat<F32> s = Stat<F32>::none();
+    for (int c = 0; c < a.chunks; c++) {
+        const f4 p = *(const f4*)(a.part + 4 * ((size_t)row * a.chunks + c));
+        Stat<F32> o;
+        o.m = p[0];
+        o.r = p[1];
+        o.z = p[2];
+        o.t = p[3];
+        s.join(o);
+    }
+    __syncthreads();
+    rank_keys(keys, n, a.n_top, top);
+    __syncthreads();
+    finish<F32>(a, row, s, top);
+}
+
 }  // namespace
 
+// Chunks of a row: enough workgroups for two to a CU, and no more than one for
+// each batch of a row.
+LogprobPlan logprobs_plan(int rows, int V, int n_top) {
+    LogprobPlan p;
+    const int64_t batches = ((int64_t)V + kBatch - 1) / kBatch;
+    int64_t chunks = rows >= 512 ? 1 : (512 + rows - 1) / rows;
+    if (chunks > batches) chunks = batches;
+    if (chunks > kMaxChunks) chunks = kMaxChunks;
+    const int64_t per = (batches + chunks - 1) / chunks;
+    p.chunks = (int)((batches + per - 1) / per);
+    p.chunk = per * kBatch < V ? (int)(per * kBatch) : V;
+    if (p.chunks > 1) {
+        p.part_bytes = align256((size_t)rows * p.chunks * 4 * sizeof(float));
+        p.ws_bytes = p.part_bytes + (size_t)rows * p.chunks * n_top * sizeof(uint64_t);
+    }
+    return p;
+}
+
 tlhip_status launch_logprobs(hipStream_t s, const LogprobArgs& a) {
-    if (a.f32) logprobs_kernel<true><<<a.rows, 256, 0, s>>>(a);
-    else logprobs_kernel<false><<<a.rows, 256, 0, s>>>(a);
+    const unsigned wg = (unsigned)a.rows * a.chunks;
+    if (a.f32) {
+        if (a.n_top) logprobs_kernel<true, true><<<wg, 256, 0, s>>>(a);
+        else logprobs_kernel<true, false><<<wg, 256, 0, s>>>(a);
+        if (a.chunks > 1) logprobs_join_kernel<true><<<a.rows, 256, 0, s>>>(a);
+    } else {
+        if (a.n_top) logprobs_kernel<false, true><<<wg, 256, 0, s>>>(a);
+        else logprobs_kernel<false, false><<<wg, 256, 0, s>>>(a);
+        if (a.chunks > 1) logprobs_join_kernel<false><<<a.rows, 256, 0, s>>>(a);
+    }
     return TLHIP_OK;
 }
 

@@ -14,7 +14,7 @@ extern "C" tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits,
     if (logits->ndim != 1 && logits->ndim != 2)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: expects [V] or [rows, V] logits, got %s", op, shape_str(logits).c_str());
     const int64_t V = last_dim(logits), rows = logits->ndim == 2 ? logits->shape[0] : 1;
-    if (V < 1 || V > INT32_MAX || rows > INT32_MAX)
+    if (V < 1 || V > (1 << 30) || rows > INT32_MAX)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: logits %s", op, shape_str(logits).c_str());
     if (n_top < 0 || n_top > kMaxTop || n_top > V)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: n_top %d not in 0..min(%d, %lld)", op, n_top, kMaxTop, (long long)V);
@@ -52,6 +52,15 @@ extern "C" tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits,
     a.n_top = n_top;
     a.f32 = logits->dtype == TLHIP_F32;
     DeviceScope scope(ctx->device);
+    const LogprobPlan pl = logprobs_plan(a.rows, a.V, n_top);
+    a.chunks = pl.chunks;
+    a.chunk = pl.chunk;
+    if (pl.ws_bytes) {
+        uint8_t* ws = (uint8_t*)ctx_workspace(ctx, pl.ws_bytes);
+        if (!ws) return fail(TLHIP_ERR_ALLOCATION, "%s: no workspace of %zu bytes", op, pl.ws_bytes);
+        a.part = (float*)ws;
+        a.part_keys = (uint64_t*)(ws + pl.part_bytes);
+    }
     TLHIP_TRY(launch_logprobs(ctx->stream, a));
     return after_launch(ctx, op);
 } TLHIP_CATCH_STATUS
