@@ -483,6 +483,8 @@ struct MoeArgs {
     int32_t* ids = nullptr;           // workspace: [M, top] chosen experts
     float* g = nullptr;               // [M, top] their weights
     float* h = nullptr;               // [M * top, I]
+    float* hmax = nullptr;            // [M * top, I / 16] largest |h| of 16
+    float* part = nullptr;            // [M * top, K] each choice's share of y
     int M = 0, K = 0, I = 0, E = 0, top = 0, normalize = 0;
     int wt_gu = 0, wt_down = 0;
 };

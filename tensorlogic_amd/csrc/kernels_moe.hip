@@ -7,6 +7,23 @@
 //
 // Weights are the f16 values that their packed types stand for, as in
 // linear(); everything between x and y is f32, rounded once.
+//
+// Four launches: the router (a workgroup per token); gate and up; down; the
+// sum over a token's experts.  What bounds the middle two is reading the
+// weights of the experts that some token chose, so each is read once: a
+// workgroup takes 16 rows of one expert (of gate and of up both), finds that
+// expert's tokens, and multiplies by all of them on the matrix cores
+// (v_mfma_f32_16x16x32_f16, A = 16 weight rows x 32 k, B = 32 k x 16 columns;
+// unused columns cost nothing that is scarce).  Its eight waves share out k
+// and add up through LDS.
+//
+// A lane's 16-byte weight load is one Q4_0 block (half a Q8_0 block, eight f16
+// values), from which it supplies A's 8-element pieces in whatever order the
+// unpacking leaves them: the columns are laid out in LDS in that order.
+//
+// The product after the activation takes h, f32, as two f16 columns, h 2^-e =
+// hi + lo, with the power of two that puts the token's largest |h| just below
+// 2^15: 22 bits of every h, and none lost to the range of f16.
 #include <cmath>
 
 #include "device_common.hpp"
@@ -16,24 +33,45 @@ namespace tlhip {
 
 namespace {
 
-template <int WT>
-__device__ __forceinline__ float weight(const void* w, const uint16_t* d, int64_t row, int K, int k) {
-    if constexpr (WT == TLHIP_F16) return h2f(((const uint16_t*)w)[row * K + k]);
-    const float s = h2f(d[row * (K / 32) + k / 32]);
-    if constexpr (WT == TLHIP_Q8_0) return (float)(h16)((float)((const int8_t*)w)[row * K + k] * s);
-    const uint8_t b = ((const uint8_t*)w)[row * (K / 2) + k / 32 * 16 + k % 16];
-    return (float)(h16)((float)((k & 16 ? b >> 4 : b & 15) - 8) * s);
-}
+constexpr int kWaves = 8;                  // of a workgroup of the products
+constexpr int kStageBytes = 64 << 10;      // columns staged in LDS at a time
+constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
 
-// A workgroup per token: the logits, the chosen experts and their weights.
-__global__ __launch_bounds__(256) void moe_router_kernel(MoeArgs a) {
+// ---------------------------------------------------------------------------
+// router
+// ---------------------------------------------------------------------------
+// A workgroup of 16 waves per token: (expert, part of K) tasks over the
+// waves, then one wave ranks.  Bound by latency.
+__global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
     __shared__ float lg[kMoeMaxExperts];
+    __shared__ float part[16];
     const int m = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int e = wave; e < a.E; e += 4) {
+    // waves per expert: all 16 waves have work when there are fewer experts
+    const int P = a.E <= 2 ? 8 : a.E <= 4 ? 4 : a.E <= 8 ? 2 : 1;
+    const uint16_t* x = a.x + (size_t)m * a.K;
+    const int pieces = a.K / 8, share = (pieces + P - 1) / P;
+    for (int task = wave; task < a.E * P; task += 16) {
+        const int e = task / P, k0 = (task % P) * share, k1 = k0 + share < pieces ? k0 + share : pieces;
+        const uint16_t* r = a.router + (size_t)e * a.K;
         float s = 0.0f;
-        for (int k = lane; k < a.K; k += 64) s = fmaf(h2f(a.x[(size_t)m * a.K + k]), h2f(a.router[(size_t)e * a.K + k]), s);
+#pragma unroll 4
+        for (int k = k0 + lane; k < k1; k += 64) {
+            const u4 xv = *(const u4*)(x + 8 * k), rv = *(const u4*)(r + 8 * k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const h2 p = as_h2(xv[i]), q = as_h2(rv[i]);
+                s = fmaf((float)p[0], (float)q[0], s);
+                s = fmaf((float)p[1], (float)q[1], s);
+            }
+        }
         s = wave_sum<64>(s);
-        if (lane == 0) lg[e] = s;
+        if (lane == 0) (P == 1 ? lg : part)[task] = s;
+    }
+    __syncthreads();
+    if (P > 1 && (int)threadIdx.x < a.E) {
+        float s = 0.0f;
+        for (int i = 0; i < P; i++) s += part[threadIdx.x * P + i];
+        lg[threadIdx.x] = s;
     }
     __syncthreads();
     if (wave) return;
@@ -84,52 +122,314 @@ __global__ __launch_bounds__(256) void moe_router_kernel(MoeArgs a) {
     }
 }
 
-// A wave per (token and choice, row of gate and up).
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+// One lane's weights of one step: a block of 32 (Q types), or 8 values of each
+// of four blocks (f16).  sub(j) is its part of A in the j-th of the step's
+// four matrix instructions.
 template <int WT>
-__global__ __launch_bounds__(256) void moe_gate_up_kernel(MoeArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (int64_t)a.M * a.top * a.I) return;
-    const int pair = (int)(at / a.I), i = (int)(at % a.I), lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)a.ids[pair] * a.I + i;
-    const uint16_t* x = a.x + (size_t)(pair / a.top) * a.K;
-    float gt = 0.0f, up = 0.0f;
-    for (int k = lane; k < a.K; k += 64) {
-        const float xv = h2f(x[k]);
-        gt = fmaf(weight<WT>(a.gate, a.gate_d, row, a.K, k), xv, gt);
-        up = fmaf(weight<WT>(a.up, a.up_d, row, a.K, k), xv, up);
+struct Weights;
+template <>
+struct Weights<TLHIP_Q4_0> {
+    u4 q;
+    uint32_t d;
+    __device__ __forceinline__ void load(const void* w, const uint16_t* wd, size_t row, int nb, int step, int g) {
+        const int b = 4 * step + g;
+        q = u4{0, 0, 0, 0};
+        d = 0;
+        if (b < nb) {
+            q = __builtin_nontemporal_load((const u4*)((const uint8_t*)w + (row * nb + b) * 16));
+            d = wd[row * nb + b];
+        }
     }
-    gt = wave_sum<64>(gt);
-    up = wave_sum<64>(up);
-    if (lane == 0) a.h[(size_t)pair * a.I + i] = a.g[pair] * (gt / (1.0f + __expf(-gt)) * up);
+    __device__ __forceinline__ h8 sub(int j) const {
+        h2 o[4];
+        q4_unpack(q[j], as_h2(d | d << 16), o);
+        return h8{o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
+    }
+};
+template <>
+struct Weights<TLHIP_Q8_0> {
+    u4 q[2];
+    uint32_t d;
+    __device__ __forceinline__ void load(const void* w, const uint16_t* wd, size_t row, int nb, int step, int g) {
+        const int b = 4 * step + g;
+        q[0] = q[1] = u4{0, 0, 0, 0};
+        d = 0;
+        if (b < nb) {
+            const u4* p = (const u4*)((const uint8_t*)w + (row * nb + b) * 32);
+            q[0] = __builtin_nontemporal_load(p);
+            q[1] = __builtin_nontemporal_load(p + 1);
+            d = wd[row * nb + b];
+        }
+    }
+    __device__ __forceinline__ h8 sub(int j) const {
+        h2 lo[2], hi[2];
+        const h2 dd = as_h2(d | d << 16);
+        q8_unpack(q[j >> 1][2 * (j & 1)], dd, lo);
+        q8_unpack(q[j >> 1][2 * (j & 1) + 1], dd, hi);
+        return h8{lo[0][0], lo[0][1], lo[1][0], lo[1][1], hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+    }
+};
+template <>
+struct Weights<TLHIP_F16> {
+    u4 q[4];
+    __device__ __forceinline__ void load(const void* w, const uint16_t*, size_t row, int nb, int step, int g) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            q[j] = u4{0, 0, 0, 0};
+            if (4 * step + j < nb) q[j] = __builtin_nontemporal_load((const u4*)((const uint16_t*)w + (row * nb + 4 * step + j) * 32 + 8 * g));
+        }
+    }
+    __device__ __forceinline__ h8 sub(int j) const { return __builtin_bit_cast(h8, q[j]); }
+};
+
+// Where the 8 elements of piece s (0..3) of a block lie, in the order of A's
+// pieces: two runs of four, at r0 and r1, each in the order 0 2 1 3 (Q types,
+// as they unpack) or 0 1 2 3 (f16).
+template <int WT>
+__device__ __forceinline__ int run0(int s) { return WT == TLHIP_Q4_0 ? 4 * s : 8 * s; }
+template <int WT>
+__device__ __forceinline__ int run1(int s) { return WT == TLHIP_Q4_0 ? 16 + 4 * s : 8 * s + 4; }
+template <int WT, typename T>
+__device__ __forceinline__ h8 piece(const T& a, const T& b) {   // f16 or f32 runs
+    if constexpr (WT == TLHIP_F16) return h8{(h16)a[0], (h16)a[1], (h16)a[2], (h16)a[3], (h16)b[0], (h16)b[1], (h16)b[2], (h16)b[3]};
+    else return h8{(h16)a[0], (h16)a[2], (h16)a[1], (h16)a[3], (h16)b[0], (h16)b[2], (h16)b[1], (h16)b[3]};
+}
+// Which piece of which block of a step lane group g needs in instruction j.
+template <int WT>
+__device__ __forceinline__ int piece_block(int j, int g) { return WT == TLHIP_F16 ? j : g; }
+template <int WT>
+__device__ __forceinline__ int piece_sub(int j, int g) { return WT == TLHIP_F16 ? g : j; }
+
+typedef h16 h4 __attribute__((ext_vector_type(4)));
+
+struct MoeShared {
+    union {
+        h8 stage[kStageBytes / 16];
+        float red[kWaves * 4 * 256];
+    };
+    int list[kTokens];      // the expert's (token, choice) pairs
+    float scale[kTokens];   // down: 2^-e of each
+    int count;
+};
+
+// Fills sh.list with the pairs that chose expert e, in order.  One wave.
+__device__ __forceinline__ void find_tokens(const MoeArgs& a, int e, MoeShared& sh) {
+    const int n = a.M * a.top, lane = threadIdx.x & 63;
+    int have = 0;
+    for (int p = 0; p < n; p += 64) {
+        const bool is = p + lane < n && a.ids[p + lane] == e;
+        const uint64_t who = __ballot(is);
+        if (is) sh.list[have + __builtin_popcountll(who & ((1ull << lane) - 1))] = p + lane;
+        have += __builtin_popcountll(who);
+    }
+    if (lane == 0) sh.count = have;
 }
 
-// A wave per output.
-template <int WT>
-__global__ __launch_bounds__(256) void moe_down_kernel(MoeArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (int64_t)a.M * a.K) return;
-    const int m = (int)(at / a.K), n = (int)(at % a.K), lane = threadIdx.x & 63;
-    float s = 0.0f;
-    for (int t = 0; t < a.top; t++) {
-        const int pair = m * a.top + t;
-        const int64_t row = (int64_t)a.ids[pair] * a.K + n;
-        for (int i = lane; i < a.I; i += 64) s = fmaf(weight<WT>(a.down, a.down_d, row, a.I, i), a.h[(size_t)pair * a.I + i], s);
+// The expert of a workgroup's slot, with sh.list and sh.count filled; -1:
+// nothing to do.  With fewer (token, choice) pairs than experts a slot is a
+// pair, and only the first pair of an expert works on it; else an expert.
+__device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared& sh) {
+    const bool by_pair = a.M * a.top < a.E;
+    const int e = by_pair ? a.ids[slot] : slot;
+    if (threadIdx.x < 64) find_tokens(a, e, sh);
+    __syncthreads();
+    return by_pair && sh.list[0] != slot ? -1 : e;
+}
+
+// acc[r][c] += W_r (16 rows from row[r], nb blocks) times the CT * 16 columns
+// of `cols` that stage() lays out chunk by chunk.
+template <int WT, int NR, int CT, typename STAGE>
+__device__ __forceinline__ void multiply(const void* const (&w)[NR], const uint16_t* const (&wd)[NR], size_t row, int nb, int ncol,
+                                         const STAGE& stage, MoeShared& sh, f4 (&acc)[NR][CT]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+    // blocks of a chunk: a multiple of what the waves take in one step
+    int chunk = kStageBytes / (64 * ncol) / (4 * kWaves) * (4 * kWaves);
+    const int all = (nb + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);
+    if (chunk > all) chunk = all;
+    int col[CT];
+#pragma unroll
+    for (int c = 0; c < CT; c++) col[c] = 16 * c + c16 < ncol ? 16 * c + c16 : ncol - 1;
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int c = 0; c < CT; c++) acc[r][c] = f4{0, 0, 0, 0};
+    Weights<WT> next[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) next[r].load(w[r], wd[r], row + c16, nb, wave, g);
+    for (int c0 = 0; c0 < nb; c0 += chunk) {
+        const int blocks = nb - c0 < chunk ? nb - c0 : chunk;
+        lds_barrier();
+        stage(c0, blocks);
+        lds_barrier();
+        for (int s = wave; 4 * s < blocks; s += kWaves) {
+            Weights<WT> cur[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                cur[r] = next[r];
+                // (chunks are whole rounds of steps, so the next step of the
+                // wave is kWaves on, in this chunk or the next)
+                next[r].load(w[r], wd[r], row + c16, nb, c0 / 4 + s + kWaves, g);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                int b = 4 * s + piece_block<WT>(j, g);
+                b = b < blocks ? b : blocks - 1;   // (A is zero there)
+                const h8* p = sh.stage + (size_t)(b * 4 + piece_sub<WT>(j, g)) * ncol;
+                h8 x[CT];
+#pragma unroll
+                for (int c = 0; c < CT; c++) x[c] = p[col[c]];
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    const h8 wv = cur[r].sub(j);
+#pragma unroll
+                    for (int c = 0; c < CT; c++) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, x[c], acc[r][c], 0, 0, 0);
+                }
+            }
+        }
     }
-    s = wave_sum<64>(s);
-    if (lane == 0) a.y[(size_t)m * a.K + n] = f2h(s);
+    // the waves' sums: red[wave][r * CT + c][col][row]
+    lds_barrier();
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int c = 0; c < CT; c++) *(f4*)(sh.red + (((wave * NR + r) * CT + c) * 16 + c16) * 16 + 4 * g) = acc[r][c];
+    lds_barrier();
+}
+template <int NR, int CT>
+__device__ __forceinline__ float summed(const MoeShared& sh, int r, int col, int row) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) s += sh.red[(((w * NR + r) * CT + (col >> 4)) * 16 + (col & 15)) * 16 + row];
+    return s;
+}
+
+// Gate and up of 16 rows of one expert, for tokens list[t0 .. t0 + nt).
+template <int WT, int CT>
+__device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int i0, int t0, int nt, MoeShared& sh) {
+    const void* const w[2] = {a.gate, a.up};
+    const uint16_t* const wd[2] = {a.gate_d, a.up_d};
+    f4 acc[2][CT];
+    auto stage = [&](int c0, int blocks) {
+        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
+            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
+            const uint16_t* x = a.x + (size_t)(sh.list[t0 + t] / a.top) * a.K + (c0 + b) * 32;
+            sh.stage[(b * 4 + s) * nt + t] = piece<WT>(*(const h4*)(x + run0<WT>(s)), *(const h4*)(x + run1<WT>(s)));
+        }
+    };
+    multiply<WT, 2, CT>(w, wd, (size_t)e * a.I + i0, a.K / 32, nt, stage, sh, acc);
+    for (int i = threadIdx.x; i < 16 * nt; i += kWaves * 64) {
+        const int row = i & 15, t = i >> 4, pair = sh.list[t0 + t];
+        const float gt = summed<2, CT>(sh, 0, t, row), up = summed<2, CT>(sh, 1, t, row);
+        const float h = a.g[pair] * (gt / (1.0f + __expf(-gt)) * up);
+        a.h[(size_t)pair * a.I + i0 + row] = h;
+        // the tile's largest |h| (a NaN counts as an infinity)
+        float m = fabsf(h) <= 3.4028235e38f ? fabsf(h) : INFINITY;
+        m = fmaxf(m, dpp_f<0xB1>(m));
+        m = fmaxf(m, dpp_f<0x4E>(m));
+        m = fmaxf(m, dpp_f<0x141>(m));
+        m = fmaxf(m, dpp_f<0x140>(m));
+        if (row == 0) a.hmax[(size_t)pair * (a.I / 16) + i0 / 16] = m;
+    }
+}
+
+template <int WT>
+__global__ __launch_bounds__(kWaves * 64) void moe_gate_up_kernel(MoeArgs a) {
+    __shared__ MoeShared sh;
+    const int tiles = a.I / 16, i0 = (int)(blockIdx.x % tiles) * 16;
+    const int e = slot_expert(a, blockIdx.x / tiles, sh);
+    if (e < 0) return;
+    const int count = sh.count;
+    for (int t0 = 0; t0 < count; t0 += 32) {
+        const int nt = count - t0 < 32 ? count - t0 : 32;
+        if (nt <= 16) gate_up_tile<WT, 1>(a, e, i0, t0, nt, sh);
+        else gate_up_tile<WT, 2>(a, e, i0, t0, nt, sh);
+        __syncthreads();
+    }
+}
+
+// Down: 16 rows of one expert; the columns are the hi and lo parts of each
+// token's h, one after the other.
+template <int WT, int CT>
+__device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int n0, int t0, int nt, MoeShared& sh) {
+    const void* const w[1] = {a.down};
+    const uint16_t* const wd[1] = {a.down_d};
+    f4 acc[1][CT];
+    auto stage = [&](int c0, int blocks) {
+        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
+            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
+            const float* h = a.h + (size_t)sh.list[t0 + t] * a.I + (c0 + b) * 32;
+            const float f = sh.scale[t0 + t];
+            const f4 p = *(const f4*)(h + run0<WT>(s)) * f, q = *(const f4*)(h + run1<WT>(s)) * f;
+            f4 pl, ql;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                pl[k] = p[k] - (float)(h16)p[k];
+                ql[k] = q[k] - (float)(h16)q[k];
+            }
+            h8* dst = sh.stage + (size_t)(b * 4 + s) * (2 * nt) + 2 * t;
+            dst[0] = piece<WT>(p, q);
+            dst[1] = piece<WT>(pl, ql);
+        }
+    };
+    multiply<WT, 1, CT>(w, wd, (size_t)e * a.K + n0, a.I / 32, 2 * nt, stage, sh, acc);
+    for (int i = threadIdx.x; i < 16 * nt; i += kWaves * 64) {
+        const int row = i & 15, t = i >> 4;
+        const float v = (summed<1, CT>(sh, 0, 2 * t, row) + summed<1, CT>(sh, 0, 2 * t + 1, row)) / sh.scale[t0 + t];
+        a.part[(size_t)sh.list[t0 + t] * a.K + n0 + row] = v;
+    }
+}
+
+template <int WT>
+__global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a) {
+    __shared__ MoeShared sh;
+    const int tiles = a.K / 16, n0 = (int)(blockIdx.x % tiles) * 16;
+    const int e = slot_expert(a, blockIdx.x / tiles, sh);
+    if (e < 0) return;
+    const int count = sh.count, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int t = wave; t < count; t += kWaves) {
+        const float* hm = a.hmax + (size_t)sh.list[t] * (a.I / 16);
+        float m = 0.0f;
+        for (int i = lane; i < a.I / 16; i += 64) m = fmaxf(m, hm[i]);
+        m = wave_max(m);
+        // 2^-e with m 2^-e in [2^14, 2^15); 1 for zeros and the non-finite
+        if (lane == 0) sh.scale[t] = m > 0.0f && m < INFINITY ? ldexpf(1.0f, min(14 - ilogbf(m), 126)) : 1.0f;
+    }
+    __syncthreads();
+    for (int t0 = 0; t0 < count; t0 += 16) {
+        const int nt = count - t0 < 16 ? count - t0 : 16;
+        if (nt <= 8) down_tile<WT, 1>(a, e, n0, t0, nt, sh);
+        else down_tile<WT, 2>(a, e, n0, t0, nt, sh);
+        __syncthreads();
+    }
+}
+
+// y = the sum of a token's experts.
+__global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
+    const int at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= a.M * (a.K / 4)) return;
+    const int m = at / (a.K / 4), n = at % (a.K / 4) * 4;
+    f4 s = {0, 0, 0, 0};
+    for (int t = 0; t < a.top; t++) s += *(const f4*)(a.part + ((size_t)m * a.top + t) * a.K + n);
+    uint16_t* y = a.y + (size_t)m * a.K + n;
+    *(uint64_t*)y = (uint64_t)f2h(s[0]) | (uint64_t)f2h(s[1]) << 16 | (uint64_t)f2h(s[2]) << 32 | (uint64_t)f2h(s[3]) << 48;
 }
 
 }  // namespace
 
 tlhip_status launch_moe(hipStream_t s, const MoeArgs& a) {
-    moe_router_kernel<<<a.M, 256, 0, s>>>(a);
-    const unsigned gu = (unsigned)(((int64_t)a.M * a.top * a.I + 3) / 4), dn = (unsigned)(((int64_t)a.M * a.K + 3) / 4);
-    if (a.wt_gu == TLHIP_F16) moe_gate_up_kernel<TLHIP_F16><<<gu, 256, 0, s>>>(a);
-    else if (a.wt_gu == TLHIP_Q4_0) moe_gate_up_kernel<TLHIP_Q4_0><<<gu, 256, 0, s>>>(a);
-    else moe_gate_up_kernel<TLHIP_Q8_0><<<gu, 256, 0, s>>>(a);
-    if (a.wt_down == TLHIP_F16) moe_down_kernel<TLHIP_F16><<<dn, 256, 0, s>>>(a);
-    else if (a.wt_down == TLHIP_Q4_0) moe_down_kernel<TLHIP_Q4_0><<<dn, 256, 0, s>>>(a);
-    else moe_down_kernel<TLHIP_Q8_0><<<dn, 256, 0, s>>>(a);
+    moe_router_kernel<<<a.M, 1024, 0, s>>>(a);
+    const unsigned slots = a.M * a.top < a.E ? a.M * a.top : a.E;
+    const unsigned gu = slots * (a.I / 16), dn = slots * (a.K / 16);
+    if (a.wt_gu == TLHIP_F16) moe_gate_up_kernel<TLHIP_F16><<<gu, kWaves * 64, 0, s>>>(a);
+    else if (a.wt_gu == TLHIP_Q4_0) moe_gate_up_kernel<TLHIP_Q4_0><<<gu, kWaves * 64, 0, s>>>(a);
+    else moe_gate_up_kernel<TLHIP_Q8_0><<<gu, kWaves * 64, 0, s>>>(a);
+    if (a.wt_down == TLHIP_F16) moe_down_kernel<TLHIP_F16><<<dn, kWaves * 64, 0, s>>>(a);
+    else if (a.wt_down == TLHIP_Q4_0) moe_down_kernel<TLHIP_Q4_0><<<dn, kWaves * 64, 0, s>>>(a);
+    else moe_down_kernel<TLHIP_Q8_0><<<dn, kWaves * 64, 0, s>>>(a);
+    moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
     return TLHIP_OK;
 }
 

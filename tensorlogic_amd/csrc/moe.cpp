@@ -54,8 +54,11 @@ extern "C" tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor ro
         return fail(TLHIP_ERR_INVALID_DIMENSION, "moe: rows of %lld and %lld (multiples of 32)", (long long)K, (long long)I);
     if (M == 0) return TLHIP_OK;
     const int64_t slab = M < kSlab ? M : kSlab;
-    const size_t ids = align256((size_t)slab * top_k * sizeof(int32_t)), g = align256((size_t)slab * top_k * sizeof(float));
-    const size_t need = ids + g + (size_t)slab * top_k * I * sizeof(float);
+    // ids, g, h, hmax, part: one after another
+    const size_t pairs = (size_t)slab * top_k;
+    const size_t at_g = align256(pairs * sizeof(int32_t)), at_h = at_g + align256(pairs * sizeof(float));
+    const size_t at_max = at_h + align256(pairs * I * sizeof(float)), at_part = at_max + align256(pairs * (I / 16) * sizeof(float));
+    const size_t need = at_part + pairs * K * sizeof(float);
     DeviceScope scope(ctx->device);
     uint8_t* ws = (uint8_t*)ctx_workspace(ctx, need);
     if (!ws) return fail(TLHIP_ERR_ALLOCATION, "moe: no workspace of %zu bytes", need);
@@ -68,8 +71,10 @@ extern "C" tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor ro
     a.up_d = up->scales;
     a.down_d = down->scales;
     a.ids = (int32_t*)ws;
-    a.g = (float*)(ws + ids);
-    a.h = (float*)(ws + ids + g);
+    a.g = (float*)(ws + at_g);
+    a.h = (float*)(ws + at_h);
+    a.hmax = (float*)(ws + at_max);
+    a.part = (float*)(ws + at_part);
     a.K = (int)K;
     a.I = (int)I;
     a.E = (int)E;
