@@ -33,8 +33,8 @@ namespace tlhip {
 
 namespace {
 
-constexpr int kWaves = 8;                  // of a workgroup of the products
-constexpr int kStageBytes = 64 << 10;      // columns staged in LDS at a time
+constexpr int kWaves = 4;                  // of a workgroup of the products
+constexpr int kStageBytes = 32 << 10;      // columns staged in LDS at a time
 constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
 
 // ---------------------------------------------------------------------------
@@ -75,41 +75,40 @@ __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
     }
     __syncthreads();
     if (wave) return;
-    float v[kMoeMaxExperts / 64], big = -INFINITY, z = 0.0f;
+    constexpr int NJ = kMoeMaxExperts / 64;
+    float v[NJ], big = -INFINITY, z = 0.0f;
     bool nan = false;
 #pragma unroll
-    for (int j = 0; j < kMoeMaxExperts / 64; j++) {
+    for (int j = 0; j < NJ; j++) {
         const int e = lane + 64 * j;
         v[j] = e < a.E ? lg[e] : -INFINITY;
         nan |= v[j] != v[j];
         big = fmaxf(big, v[j]);
     }
-    nan = __any(nan);
+    nan = __any(nan);   // (then any experts will do: their weights are NaN)
     big = wave_max(big);
 #pragma unroll
-    for (int j = 0; j < kMoeMaxExperts / 64; j++) z += lane + 64 * j < a.E ? __builtin_amdgcn_exp2f((v[j] - big) * 1.44269504f) : 0.0f;
+    for (int j = 0; j < NJ; j++) z += lane + 64 * j < a.E ? __builtin_amdgcn_exp2f((v[j] - big) * 1.44269504f) : 0.0f;
     z = wave_sum<64>(z);
-    // rounds of the largest (value, lowest index); a chosen one leaves.  NaN
-    // ranks below everything, so every round finds an expert.
+    // rounds of the largest value, at its lowest index; a chosen one leaves
     float chosen = 0.0f, mine = 0.0f;
-    uint32_t gone = 0;
-    int id = 0;
-    for (int t = 0; t < a.top; t++) {
-        uint64_t best = 0;
+    uint32_t gone = 0;   // bit j: expert lane + 64 j is chosen, or none
+    int id = lane;
 #pragma unroll
-        for (int j = 0; j < kMoeMaxExperts / 64; j++) {
-            const uint32_t e = lane + 64 * j, b = __float_as_uint(v[j] + 0.0f);
-            const uint32_t o = v[j] != v[j] ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
-            const uint64_t k = e < (uint32_t)a.E && !(gone >> j & 1) ? (uint64_t)o << 32 | (0xFFFFFFFFu - e) : 0;
-            best = k > best ? k : best;
+    for (int j = 0; j < NJ; j++) gone |= (lane + 64 * j >= a.E ? 1u : 0u) << j;
+    for (int t = 0; t < a.top && !nan; t++) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) top = fmaxf(top, gone >> j & 1 ? -INFINITY : v[j]);
+        top = wave_max(top);
+        int e = 0;
+#pragma unroll
+        for (int j = NJ - 1; j >= 0; j--) {
+            const uint64_t who = __ballot(!(gone >> j & 1) && v[j] == top);
+            if (who) e = 64 * j + __builtin_ctzll(who);
         }
-        for (int k = 32; k; k >>= 1) {
-            const uint64_t o = __shfl_xor((unsigned long long)best, k, 64);
-            best = o > best ? o : best;
-        }
-        const int e = (int)(0xFFFFFFFFu - (uint32_t)best);
         if ((e & 63) == lane) gone |= 1u << (e >> 6);
-        const float p = __builtin_amdgcn_exp2f((lg[e] - big) * 1.44269504f);
+        const float p = __builtin_amdgcn_exp2f((top - big) * 1.44269504f);
         chosen += p;
         if (lane == t) {
             id = e;
@@ -232,6 +231,14 @@ __device__ __forceinline__ void find_tokens(const MoeArgs& a, int e, MoeShared& 
 // nothing to do.  With fewer (token, choice) pairs than experts a slot is a
 // pair, and only the first pair of an expert works on it; else an expert.
 __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared& sh) {
+    if (a.M == 1 && a.top < a.E) {
+        if (threadIdx.x == 0) {
+            sh.list[0] = slot;
+            sh.count = 1;
+        }
+        __syncthreads();
+        return a.ids[slot];
+    }
     const bool by_pair = a.M * a.top < a.E;
     const int e = by_pair ? a.ids[slot] : slot;
     if (threadIdx.x < 64) find_tokens(a, e, sh);
@@ -256,9 +263,12 @@ __device__ __forceinline__ void multiply(const void* const (&w)[NR], const uint1
     for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int c = 0; c < CT; c++) acc[r][c] = f4{0, 0, 0, 0};
-    Weights<WT> next[NR];
+    constexpr int PD = WT == TLHIP_Q4_0 ? 5 - NR : WT == TLHIP_Q8_0 ? 4 - NR : 3 - NR;   // steps loaded ahead
+    Weights<WT> ring[PD][NR];
 #pragma unroll
-    for (int r = 0; r < NR; r++) next[r].load(w[r], wd[r], row + c16, nb, wave, g);
+    for (int k = 0; k < PD; k++)
+#pragma unroll
+        for (int r = 0; r < NR; r++) ring[k][r].load(w[r], wd[r], row + c16, nb, wave + k * kWaves, g);
     for (int c0 = 0; c0 < nb; c0 += chunk) {
         const int blocks = nb - c0 < chunk ? nb - c0 : chunk;
         lds_barrier();
@@ -268,10 +278,12 @@ __device__ __forceinline__ void multiply(const void* const (&w)[NR], const uint1
             Weights<WT> cur[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                cur[r] = next[r];
-                // (chunks are whole rounds of steps, so the next step of the
-                // wave is kWaves on, in this chunk or the next)
-                next[r].load(w[r], wd[r], row + c16, nb, c0 / 4 + s + kWaves, g);
+                cur[r] = ring[0][r];
+#pragma unroll
+                for (int k = 1; k < PD; k++) ring[k - 1][r] = ring[k][r];
+                // (chunks are whole rounds of steps, so the wave's later steps
+                // are kWaves apart in this chunk and the next)
+                ring[PD - 1][r].load(w[r], wd[r], row + c16, nb, c0 / 4 + s + PD * kWaves, g);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -406,6 +418,72 @@ __global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a) {
     }
 }
 
+// Down for a single token: all its experts in one workgroup per 16 rows, so
+// that no sum is left over.  Sixteen waves share out the (expert, step) pairs;
+// the columns are hi and lo of h under one power of two.
+constexpr int kOneSteps = 64;   // steps of 4 blocks staged at a time (32 KB)
+template <int WT>
+__global__ __launch_bounds__(1024) void moe_down_one_kernel(MoeArgs a) {
+    __shared__ h8 stage[kOneSteps * 32];
+    __shared__ float red[16][2][16], most[16];
+    constexpr int PD = WT == TLHIP_F16 ? 1 : 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + 3) / 4, steps = a.top * per;
+    const int ids = a.ids[lane < a.top ? lane : 0];
+    auto load = [&](Weights<WT>& w, int n) {
+        const int t = n < steps ? n / per : 0, e = __builtin_amdgcn_readlane(ids, t);
+        // (past the last step: a step past the row's end, which loads nothing)
+        w.load(a.down, a.down_d, (size_t)e * a.K + n0 + c16, nb, n < steps ? n - t * per : per, g);
+    };
+    Weights<WT> ring[PD];
+#pragma unroll
+    for (int k = 0; k < PD; k++) load(ring[k], wave + 16 * k);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < a.top * (a.I / 16); i += 1024) m = fmaxf(m, a.hmax[i]);
+    m = block_max1<16>(m, most);
+    const float scale = m > 0.0f && m < INFINITY ? ldexpf(1.0f, min(14 - ilogbf(m), 126)) : 1.0f;
+    f4 acc = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < steps; s0 += kOneSteps) {
+        const int n1 = steps - s0 < kOneSteps ? steps - s0 : kOneSteps;
+        lds_barrier();
+        for (int i = threadIdx.x; i < n1 * 16; i += 1024) {
+            const int s = i & 3, b = i >> 2, n = s0 + (b >> 2), t = n / per, block = 4 * (n - t * per) + (b & 3);
+            f4 p = {0, 0, 0, 0}, q = p, pl, ql;
+            if (block < nb) {
+                const float* h = a.h + (size_t)t * a.I + block * 32;
+                p = *(const f4*)(h + run0<WT>(s)) * scale;
+                q = *(const f4*)(h + run1<WT>(s)) * scale;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                pl[k] = p[k] - (float)(h16)p[k];
+                ql[k] = q[k] - (float)(h16)q[k];
+            }
+            stage[2 * i] = piece<WT>(p, q);
+            stage[2 * i + 1] = piece<WT>(pl, ql);
+        }
+        lds_barrier();
+        for (int n = wave; n < n1; n += 16) {
+            const Weights<WT> cur = ring[0];
+#pragma unroll
+            for (int k = 1; k < PD; k++) ring[k - 1] = ring[k];
+            load(ring[PD - 1], s0 + n + 16 * PD);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const h8 x = stage[((4 * n + piece_block<WT>(j, g)) * 4 + piece_sub<WT>(j, g)) * 2 + (c16 & 1)];
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(cur.sub(j), x, acc, 0, 0, 0);
+            }
+        }
+    }
+    if (c16 < 2) *(f4*)&red[wave][c16][4 * g] = acc;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float s = 0.0f;
+        for (int w = 0; w < 16; w++) s += red[w][0][threadIdx.x] + red[w][1][threadIdx.x];
+        a.y[n0 + threadIdx.x] = f2h(s / scale);
+    }
+}
+
 // y = the sum of a token's experts.
 __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
     const int at = blockIdx.x * 256 + threadIdx.x;
@@ -419,17 +497,29 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 
 }  // namespace
 
+template <int WT>
+static void launch_gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    moe_gate_up_kernel<WT><<<slots * (a.I / 16), kWaves * 64, 0, s>>>(a);
+}
+template <int WT>
+static void launch_down(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    if (a.M == 1) {
+        moe_down_one_kernel<WT><<<a.K / 16, 1024, 0, s>>>(a);
+        return;
+    }
+    moe_down_kernel<WT><<<slots * (a.K / 16), kWaves * 64, 0, s>>>(a);
+    moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
+}
+
 tlhip_status launch_moe(hipStream_t s, const MoeArgs& a) {
     moe_router_kernel<<<a.M, 1024, 0, s>>>(a);
     const unsigned slots = a.M * a.top < a.E ? a.M * a.top : a.E;
-    const unsigned gu = slots * (a.I / 16), dn = slots * (a.K / 16);
-    if (a.wt_gu == TLHIP_F16) moe_gate_up_kernel<TLHIP_F16><<<gu, kWaves * 64, 0, s>>>(a);
-    else if (a.wt_gu == TLHIP_Q4_0) moe_gate_up_kernel<TLHIP_Q4_0><<<gu, kWaves * 64, 0, s>>>(a);
-    else moe_gate_up_kernel<TLHIP_Q8_0><<<gu, kWaves * 64, 0, s>>>(a);
-    if (a.wt_down == TLHIP_F16) moe_down_kernel<TLHIP_F16><<<dn, kWaves * 64, 0, s>>>(a);
-    else if (a.wt_down == TLHIP_Q4_0) moe_down_kernel<TLHIP_Q4_0><<<dn, kWaves * 64, 0, s>>>(a);
-    else moe_down_kernel<TLHIP_Q8_0><<<dn, kWaves * 64, 0, s>>>(a);
-    moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
+    if (a.wt_gu == TLHIP_F16) launch_gate_up<TLHIP_F16>(s, a, slots);
+    else if (a.wt_gu == TLHIP_Q4_0) launch_gate_up<TLHIP_Q4_0>(s, a, slots);
+    else launch_gate_up<TLHIP_Q8_0>(s, a, slots);
+    if (a.wt_down == TLHIP_F16) launch_down<TLHIP_F16>(s, a, slots);
+    else if (a.wt_down == TLHIP_Q4_0) launch_down<TLHIP_Q4_0>(s, a, slots);
+    else launch_down<TLHIP_Q8_0>(s, a, slots);
     return TLHIP_OK;
 }
 
