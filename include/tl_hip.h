@@ -297,7 +297,7 @@ tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tens
  * x and y [M, K], router [E, K], all f16; gate and up [E * I, K] and down
  * [E * K, I], the experts' rows one after another (f16 also [E, I, K] and
  * [E, K, I]), each F16, Q4_0 or Q8_0, gate and up of one type.  K and I are
- * multiples of 32, E <= 256, top_k <= min(E, 32).  The weights count as the
+ * multiples of 32 up to 16384, E <= 256, top_k <= min(E, 32).  The weights count as the
  * f16 values that linear() reads them as; what lies between x and y is not
  * rounded to f16.  y may be x.  Any M; the weights an expert's tokens need
  * are read once for up to 256 tokens.                                      */

@@ -488,7 +488,7 @@ struct MoeArgs {
     int M = 0, K = 0, I = 0, E = 0, top = 0, normalize = 0;
     int wt_gu = 0, wt_down = 0;
 };
-constexpr int kMoeMaxExperts = 256, kMoeMaxTop = 32;
+constexpr int kMoeMaxExperts = 256, kMoeMaxTop = 32, kMoeMaxRow = 16384;
 tlhip_status launch_moe(hipStream_t s, const MoeArgs& a);
 
 tlhip_status launch_copy_rows(hipStream_t s, const uint16_t* src, uint16_t* dst, int rows,

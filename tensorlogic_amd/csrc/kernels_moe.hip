@@ -9,17 +9,20 @@
 // linear(); everything between x and y is f32, rounded once.
 //
 // Four launches: the router (a workgroup per token); gate and up; down; the
-// sum over a token's experts.  What bounds the middle two is reading the
-// weights of the experts that some token chose, so each is read once: a
-// workgroup takes 16 rows of one expert (of gate and of up both), finds that
-// expert's tokens, and multiplies by all of them on the matrix cores
-// (v_mfma_f32_16x16x32_f16, A = 16 weight rows x 32 k, B = 32 k x 16 columns;
-// unused columns cost nothing that is scarce).  Its eight waves share out k
-// and add up through LDS.
+// sum over a token's experts (three for one token, whose down sums them
+// itself).  What bounds the middle two is reading the weights of the experts
+// that some token chose, so each is read once: a wave takes 16 rows of one
+// expert (of gate and of up both) and multiplies by all of that expert's
+// tokens on the matrix cores (v_mfma_f32_16x16x32_f16, A = 16 weight rows x 32
+// k, B = 32 k x 16 columns; unused columns cost nothing that is scarce).
 //
-// A lane's 16-byte weight load is one Q4_0 block (half a Q8_0 block, eight f16
-// values), from which it supplies A's 8-element pieces in whatever order the
-// unpacking leaves them: the columns are laid out in LDS in that order.
+// The weights go through LDS, copied there directly (no registers) in slots
+// of 16 rows x 128 bytes (f16: 256): whole cache lines, where A's own layout
+// asks for 64 bytes of each of 16 rows at a time.  Through registers in that
+// layout, and with the 2-byte scales gathered one by one, 13 Q8_0 tokens' gate
+// and up of 5632 x 2048 took 55 us (3.5 TB/s) without any arithmetic.  A tile's
+// scales lie together and are copied whole.  Each wave has its own ring of
+// slots, so its stream of loads waits for no other.
 //
 // The product after the activation takes h, f32, as two f16 columns, h 2^-e =
 // hi + lo, with the power of two that puts the token's largest |h| just below
@@ -34,12 +37,24 @@ namespace tlhip {
 namespace {
 
 constexpr int kWaves = 4;                  // of a workgroup of the products
-constexpr int kStageBytes = 32 << 10;      // columns staged in LDS at a time
+constexpr int kColumnBytes = 32 << 10;     // columns staged in LDS at a time (or one round of slots, if that is more)
 constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
+constexpr int kRing = 2;                   // slots of weights a wave has in flight
 
 // ---------------------------------------------------------------------------
 // router
 // ---------------------------------------------------------------------------
+// The wave's maximum without the LDS round trips of a shuffle.
+__device__ __forceinline__ float wave_max_u(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    v = fmaxf(v, dpp_f<0x140>(v));
+    const int b = __float_as_int(v);
+    return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(b, 0)), __int_as_float(__builtin_amdgcn_readlane(b, 16))),
+                 fmaxf(__int_as_float(__builtin_amdgcn_readlane(b, 32)), __int_as_float(__builtin_amdgcn_readlane(b, 48))));
+}
+
 // A workgroup of 16 waves per token: (expert, part of K) tasks over the
 // waves, then one wave ranks.  Bound by latency.
 __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
@@ -86,7 +101,7 @@ __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
         big = fmaxf(big, v[j]);
     }
     nan = __any(nan);   // (then any experts will do: their weights are NaN)
-    big = wave_max(big);
+    big = wave_max_u(big);
 #pragma unroll
     for (int j = 0; j < NJ; j++) z += lane + 64 * j < a.E ? __builtin_amdgcn_exp2f((v[j] - big) * 1.44269504f) : 0.0f;
     z = wave_sum<64>(z);
@@ -100,7 +115,7 @@ __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NJ; j++) top = fmaxf(top, gone >> j & 1 ? -INFINITY : v[j]);
-        top = wave_max(top);
+        top = wave_max_u(top);
         int e = 0;
 #pragma unroll
         for (int j = NJ - 1; j >= 0; j--) {
@@ -124,23 +139,31 @@ __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
 // ---------------------------------------------------------------------------
 // products
 // ---------------------------------------------------------------------------
-// One lane's weights of one step: a block of 32 (Q types), or 8 values of each
-// of four blocks (f16).  sub(j) is its part of A in the j-th of the step's
-// four matrix instructions.
+// A slot: RB bytes of each of 16 rows, STEPS steps of four blocks of 32.  The
+// 16-byte piece at place q of a row is the row's piece q ^ swizzle(row): the 16
+// rows' reads of one piece then take 16 different places of the 256 bytes that
+// LDS gives in a cycle.
+template <int WT>
+struct Slot {
+    static constexpr int RB = WT == TLHIP_F16 ? 256 : 128, NP = RB / 16, BYTES = 16 * RB, COPIES = BYTES / 1024;
+    static constexpr int STEPS = WT == TLHIP_Q4_0 ? 2 : 1, BLOCKS = 4 * STEPS;
+    static constexpr int BLOCK_BYTES = WT == TLHIP_Q4_0 ? 16 : WT == TLHIP_Q8_0 ? 32 : 64;
+    static __device__ __forceinline__ int swizzle(int row) { return NP == 8 ? row >> 1 & 7 : row; }
+};
+
+// One lane's weights of one step: a block (Q4_0), half of each of two (Q8_0) or
+// a quarter of each of four (f16).  sub(j) is its part of A in the j-th of the
+// step's four matrix instructions.
 template <int WT>
 struct Weights;
 template <>
 struct Weights<TLHIP_Q4_0> {
     u4 q;
     uint32_t d;
-    __device__ __forceinline__ void load(const void* w, const uint16_t* wd, size_t row, int nb, int step, int g) {
-        const int b = 4 * step + g;
-        q = u4{0, 0, 0, 0};
-        d = 0;
-        if (b < nb) {
-            q = __builtin_nontemporal_load((const u4*)((const uint8_t*)w + (row * nb + b) * 16));
-            d = wd[row * nb + b];
-        }
+    __device__ __forceinline__ void read(const uint8_t* slot, const uint16_t* d16, int row, int nb, int block0, int u, int g) {
+        q = *(const u4*)(slot + row * 128 + ((4 * u + g) ^ Slot<TLHIP_Q4_0>::swizzle(row)) * 16);
+        const int b = block0 + 4 * u + g;
+        d = d16[row * nb + (b < nb ? b : nb - 1)];
     }
     __device__ __forceinline__ h8 sub(int j) const {
         h2 o[4];
@@ -151,21 +174,18 @@ struct Weights<TLHIP_Q4_0> {
 template <>
 struct Weights<TLHIP_Q8_0> {
     u4 q[2];
-    uint32_t d;
-    __device__ __forceinline__ void load(const void* w, const uint16_t* wd, size_t row, int nb, int step, int g) {
-        const int b = 4 * step + g;
-        q[0] = q[1] = u4{0, 0, 0, 0};
-        d = 0;
-        if (b < nb) {
-            const u4* p = (const u4*)((const uint8_t*)w + (row * nb + b) * 32);
-            q[0] = __builtin_nontemporal_load(p);
-            q[1] = __builtin_nontemporal_load(p + 1);
-            d = wd[row * nb + b];
+    uint32_t d[2];
+    __device__ __forceinline__ void read(const uint8_t* slot, const uint16_t* d16, int row, int nb, int block0, int, int g) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            q[i] = *(const u4*)(slot + row * 128 + ((4 * i + g) ^ Slot<TLHIP_Q8_0>::swizzle(row)) * 16);
+            const int b = block0 + 2 * i + (g >> 1);
+            d[i] = d16[row * nb + (b < nb ? b : nb - 1)];
         }
     }
     __device__ __forceinline__ h8 sub(int j) const {
         h2 lo[2], hi[2];
-        const h2 dd = as_h2(d | d << 16);
+        const h2 dd = as_h2(d[j >> 1] | d[j >> 1] << 16);
         q8_unpack(q[j >> 1][2 * (j & 1)], dd, lo);
         q8_unpack(q[j >> 1][2 * (j & 1) + 1], dd, hi);
         return h8{lo[0][0], lo[0][1], lo[1][0], lo[1][1], hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
@@ -174,12 +194,9 @@ struct Weights<TLHIP_Q8_0> {
 template <>
 struct Weights<TLHIP_F16> {
     u4 q[4];
-    __device__ __forceinline__ void load(const void* w, const uint16_t*, size_t row, int nb, int step, int g) {
+    __device__ __forceinline__ void read(const uint8_t* slot, const uint16_t*, int row, int, int, int, int g) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            q[j] = u4{0, 0, 0, 0};
-            if (4 * step + j < nb) q[j] = __builtin_nontemporal_load((const u4*)((const uint16_t*)w + (row * nb + 4 * step + j) * 32 + 8 * g));
-        }
+        for (int j = 0; j < 4; j++) q[j] = *(const u4*)(slot + row * 256 + ((4 * j + g) ^ row) * 16);
     }
     __device__ __forceinline__ h8 sub(int j) const { return __builtin_bit_cast(h8, q[j]); }
 };
@@ -198,19 +215,54 @@ __device__ __forceinline__ h8 piece(const T& a, const T& b) {   // f16 or f32 ru
 }
 // Which piece of which block of a step lane group g needs in instruction j.
 template <int WT>
-__device__ __forceinline__ int piece_block(int j, int g) { return WT == TLHIP_F16 ? j : g; }
+__device__ __forceinline__ int piece_block(int j, int g) {
+    return WT == TLHIP_F16 ? j : WT == TLHIP_Q8_0 ? 2 * (j >> 1) + (g >> 1) : g;
+}
 template <int WT>
-__device__ __forceinline__ int piece_sub(int j, int g) { return WT == TLHIP_F16 ? g : j; }
+__device__ __forceinline__ int piece_sub(int j, int g) {
+    return WT == TLHIP_F16 ? g : WT == TLHIP_Q8_0 ? 2 * (g & 1) + (j & 1) : j;
+}
 
 typedef h16 h4 __attribute__((ext_vector_type(4)));
 
+// 16 weight rows whose slots a wave copies to LDS.
+template <int WT>
+struct Rows {
+    using S = Slot<WT>;
+    __amdgpu_buffer_rsrc_t q;
+    int row_bytes;
+    __device__ __forceinline__ Rows(const void* w, size_t row, int nb)
+        : q(sk_rsrc((const uint8_t*)w + row * nb * S::BLOCK_BYTES, 16u * nb * S::BLOCK_BYTES)), row_bytes(nb * S::BLOCK_BYTES) {}
+    // Slot n to LDS address `lds`.  Pieces past the row's end repeat its last
+    // one: their columns are zero.
+    __device__ __forceinline__ void copy(int n, uint32_t lds) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < S::COPIES; i++) {
+            const int at = i * 64 + lane, row = at / S::NP, byte = n * S::RB + ((at % S::NP) ^ S::swizzle(row)) * 16;
+            sk_dma<16>(q, lds + i * 1024, row * row_bytes + (byte < row_bytes ? byte : row_bytes - 16));
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(gl_lds_t)p; }
+// This wave's LDS reads are done (their memory may be copied over).
+__device__ __forceinline__ void lds_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The scales of 16 rows (nb of them each, which lie together) to LDS, by all
+// threads of `threads`.
+__device__ __forceinline__ void copy_scales(uint16_t* dst, const uint16_t* d, size_t row, int nb, int thread, int threads) {
+    const u4* src = (const u4*)(d + row * nb);   // (16 nb values from a multiple of 16: 32-byte aligned)
+    for (int i = thread; i < 2 * nb; i += threads) ((u4*)dst)[i] = src[i];
+}
+
+// What a workgroup holds in LDS before its dynamic part, which is: columns,
+// rings, scales.
 struct MoeShared {
-    union {
-        h8 stage[kStageBytes / 16];
-        float red[kWaves * 4 * 256];
-    };
     int list[kTokens];      // the expert's (token, choice) pairs
+    float g[kTokens];       // their weights
     float scale[kTokens];   // down: 2^-e of each
+    f4 red[kWaves * 4 * 64];
     int count;
 };
 
@@ -221,7 +273,11 @@ __device__ __forceinline__ void find_tokens(const MoeArgs& a, int e, MoeShared& 
     for (int p = 0; p < n; p += 64) {
         const bool is = p + lane < n && a.ids[p + lane] == e;
         const uint64_t who = __ballot(is);
-        if (is) sh.list[have + __builtin_popcountll(who & ((1ull << lane) - 1))] = p + lane;
+        if (is) {
+            const int at = have + __builtin_popcountll(who & ((1ull << lane) - 1));
+            sh.list[at] = p + lane;
+            sh.g[at] = a.g[p + lane];
+        }
         have += __builtin_popcountll(who);
     }
     if (lane == 0) sh.count = have;
@@ -234,6 +290,7 @@ __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared
     if (a.M == 1 && a.top < a.E) {
         if (threadIdx.x == 0) {
             sh.list[0] = slot;
+            sh.g[0] = a.g[slot];
             sh.count = 1;
         }
         __syncthreads();
@@ -246,16 +303,90 @@ __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared
     return by_pair && sh.list[0] != slot ? -1 : e;
 }
 
-// acc[r][c] += W_r (16 rows from row[r], nb blocks) times the CT * 16 columns
-// of `cols` that stage() lays out chunk by chunk.
-template <int WT, int NR, int CT, typename STAGE>
-__device__ __forceinline__ void multiply(const void* const (&w)[NR], const uint16_t* const (&wd)[NR], size_t row, int nb, int ncol,
-                                         const STAGE& stage, MoeShared& sh, f4 (&acc)[NR][CT]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-    // blocks of a chunk: a multiple of what the waves take in one step
-    int chunk = kStageBytes / (64 * ncol) / (4 * kWaves) * (4 * kWaves);
-    const int all = (nb + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);
+// The columns of gate and up: x of the tokens list[0 .. nt).  Block b, piece s
+// of token t is 16 bytes at (4 b + s) * ncol + t; past the row's nb blocks zeros.
+template <int WT>
+struct StageX {
+    const MoeArgs& a;
+    const int* list;
+    int nt;
+    __device__ __forceinline__ int ncol() const { return nt; }
+    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
+        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
+            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
+            h8 v = {};
+            if (c0 + b < nb) {
+                const uint16_t* x = a.x + (size_t)(list[t] / a.top) * a.K + (c0 + b) * 32;
+                v = piece<WT>(*(const h4*)(x + run0<WT>(s)), *(const h4*)(x + run1<WT>(s)));
+            }
+            cols[(b * 4 + s) * nt + t] = v;
+        }
+    }
+};
+// Those of down: hi and lo of each token's h 2^-e.
+__device__ __forceinline__ f4 low_part(const f4& p) {
+    f4 r;
+#pragma unroll
+    for (int k = 0; k < 4; k++) r[k] = p[k] - (float)(h16)p[k];
+    return r;
+}
+template <int WT>
+struct StageH {
+    const MoeArgs& a;
+    const int* list;
+    int nt;
+    const float* scale;
+    __device__ __forceinline__ int ncol() const { return 2 * nt; }
+    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
+        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
+            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
+            f4 p = {0, 0, 0, 0}, q = p;
+            if (c0 + b < nb) {
+                const float* h = a.h + (size_t)list[t] * a.I + (c0 + b) * 32;
+                p = *(const f4*)(h + run0<WT>(s)) * scale[t];
+                q = *(const f4*)(h + run1<WT>(s)) * scale[t];
+            }
+            h8* dst = cols + (b * 4 + s) * (2 * nt) + 2 * t;
+            dst[0] = piece<WT>(p, q);
+            dst[1] = piece<WT>(low_part(p), low_part(q));
+        }
+    }
+};
+
+// Where the dynamic part of LDS holds what, for a product of nb blocks with
+// NR matrices, tiles_wg tiles in a workgroup.
+struct Layout {
+    int column_bytes, ring_at, scales_at, bytes;
+};
+template <int WT, int NR, int KS>
+__host__ __device__ inline Layout layout(int nb, int max_cols) {
+    constexpr int round = Slot<WT>::BLOCKS * KS;
+    Layout l;
+    const int whole = (nb + round - 1) / round * round * 64 * max_cols, least = round * 64 * max_cols;
+    l.column_bytes = whole < kColumnBytes ? whole : kColumnBytes > least ? kColumnBytes : least;
+    l.ring_at = l.column_bytes;
+    l.scales_at = l.ring_at + kWaves * NR * kRing * Slot<WT>::BYTES;
+    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : kWaves / KS * NR * 32 * nb);
+    return l;
+}
+
+// acc[r][c] = W_r (16 rows, nb blocks) times the CT * 16 columns that stage()
+// lays out chunk by chunk, k shared out over KS waves.  Complete in the first
+// of them: lane (c16, g) has rows 4g .. 4g + 3 of column c16.
+template <int WT, int NR, int CT, int KS, typename STAGE>
+__device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t* const (&wd)[NR], size_t row, int nb, const STAGE& stage,
+                                         const Layout& at, uint8_t* lds, MoeShared& sh, f4 (&acc)[NR][CT]) {
+    using S = Slot<WT>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS;
+    const int c16 = lane & 15, g = lane >> 4, ncol = stage.ncol();
+    constexpr int ROUND = S::BLOCKS * KS;
+    int chunk = at.column_bytes / (64 * ncol) / ROUND * ROUND;   // blocks of a chunk: whole rounds of the KS waves' slots
+    const int all = (nb + ROUND - 1) / ROUND * ROUND;
     if (chunk > all) chunk = all;
+    h8* cols = (h8*)lds;
+    const uint8_t* ring = lds + at.ring_at + wave * (NR * kRing * S::BYTES);
+    const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(ring));
+    uint16_t* scales = (uint16_t*)(lds + at.scales_at) + wave / KS * (NR * 16 * nb);
     int col[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) col[c] = 16 * c + c16 < ncol ? 16 * c + c16 : ncol - 1;
@@ -263,142 +394,167 @@ __device__ __forceinline__ void multiply(const void* const (&w)[NR], const uint1
     for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int c = 0; c < CT; c++) acc[r][c] = f4{0, 0, 0, 0};
-    constexpr int PD = WT == TLHIP_Q4_0 ? 5 - NR : WT == TLHIP_Q8_0 ? 4 - NR : 3 - NR;   // steps loaded ahead
-    Weights<WT> ring[PD][NR];
+    const int slots = (nb + S::BLOCKS - 1) / S::BLOCKS;
+    auto copy = [&](int n, int k) {   // slot n to ring place k
 #pragma unroll
-    for (int k = 0; k < PD; k++)
+        for (int r = 0; r < NR; r++) w[r].copy(n, ring_lds + (k * NR + r) * S::BYTES);
+    };
+    int next = part, place = 0;   // the next slot to copy
 #pragma unroll
-        for (int r = 0; r < NR; r++) ring[k][r].load(w[r], wd[r], row + c16, nb, wave + k * kWaves, g);
-    for (int c0 = 0; c0 < nb; c0 += chunk) {
-        const int blocks = nb - c0 < chunk ? nb - c0 : chunk;
+    for (int k = 0; k < kRing; k++, next += KS)
+        if (next < slots) copy(next, k);
+    if constexpr (WT != TLHIP_F16)
+#pragma unroll
+        for (int r = 0; r < NR; r++) copy_scales(scales + r * 16 * nb, wd[r], row, nb, threadIdx.x % (KS * 64), KS * 64);
+    for (int c0 = 0; c0 < all; c0 += chunk) {
+        const int blocks = all - c0 < chunk ? all - c0 : chunk;
         lds_barrier();
-        stage(c0, blocks);
+        stage(cols, c0, blocks, nb);
         lds_barrier();
-        for (int s = wave; 4 * s < blocks; s += kWaves) {
-            Weights<WT> cur[NR];
+        const int end = min((c0 + blocks) / S::BLOCKS, slots);
+        for (int n = c0 / S::BLOCKS + part; n < end; n += KS) {
+            // the slot has landed when no more copies are in flight than the
+            // kRing - 1 later slots'
+            if (next > n + (kRing - 1) * KS) sk_wait_vm<(kRing - 1) * NR * S::COPIES>();
+            else sk_wait_vm<0>();
+            Weights<WT> a[NR][S::STEPS];
+            const uint8_t* slot = ring + place * (NR * S::BYTES);
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                cur[r] = ring[0][r];
+            for (int r = 0; r < NR; r++)
 #pragma unroll
-                for (int k = 1; k < PD; k++) ring[k - 1][r] = ring[k][r];
-                // (chunks are whole rounds of steps, so the wave's later steps
-                // are kWaves apart in this chunk and the next)
-                ring[PD - 1][r].load(w[r], wd[r], row + c16, nb, c0 / 4 + s + PD * kWaves, g);
+                for (int u = 0; u < S::STEPS; u++) a[r][u].read(slot + r * S::BYTES, scales + r * 16 * nb, c16, nb, n * S::BLOCKS, u, g);
+            if (next < slots) {
+                lds_reads_done();
+                copy(next, place);
+                next += KS;
             }
+            place = place + 1 == kRing ? 0 : place + 1;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                int b = 4 * s + piece_block<WT>(j, g);
-                b = b < blocks ? b : blocks - 1;   // (A is zero there)
-                const h8* p = sh.stage + (size_t)(b * 4 + piece_sub<WT>(j, g)) * ncol;
-                h8 x[CT];
+            for (int u = 0; u < S::STEPS; u++) {
+                h8 x[4][CT];
 #pragma unroll
-                for (int c = 0; c < CT; c++) x[c] = p[col[c]];
+                for (int j = 0; j < 4; j++) {
+                    const int b = n * S::BLOCKS - c0 + 4 * u + piece_block<WT>(j, g);
 #pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    const h8 wv = cur[r].sub(j);
-#pragma unroll
-                    for (int c = 0; c < CT; c++) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, x[c], acc[r][c], 0, 0, 0);
+                    for (int c = 0; c < CT; c++) x[j][c] = cols[(b * 4 + piece_sub<WT>(j, g)) * ncol + col[c]];
                 }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int r = 0; r < NR; r++) {
+                        const h8 wv = a[r][u].sub(j);
+#pragma unroll
+                        for (int c = 0; c < CT; c++) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, x[j][c], acc[r][c], 0, 0, 0);
+                    }
             }
         }
     }
-    // the waves' sums: red[wave][r * CT + c][col][row]
-    lds_barrier();
+    if constexpr (KS > 1) {
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+        for (int r = 0; r < NR; r++)
 #pragma unroll
-        for (int c = 0; c < CT; c++) *(f4*)(sh.red + (((wave * NR + r) * CT + c) * 16 + c16) * 16 + 4 * g) = acc[r][c];
-    lds_barrier();
-}
-template <int NR, int CT>
-__device__ __forceinline__ float summed(const MoeShared& sh, int r, int col, int row) {
-    float s = 0.0f;
+            for (int c = 0; c < CT; c++) sh.red[((wave * NR + r) * CT + c) * 64 + lane] = acc[r][c];
+        lds_barrier();
+        if (part == 0)
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) s += sh.red[(((w * NR + r) * CT + (col >> 4)) * 16 + (col & 15)) * 16 + row];
-    return s;
+            for (int k = 1; k < KS; k++)
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int c = 0; c < CT; c++) acc[r][c] += sh.red[(((wave + k) * NR + r) * CT + c) * 64 + lane];
+    }
 }
 
 // Gate and up of 16 rows of one expert, for tokens list[t0 .. t0 + nt).
-template <int WT, int CT>
-__device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int i0, int t0, int nt, MoeShared& sh) {
-    const void* const w[2] = {a.gate, a.up};
-    const uint16_t* const wd[2] = {a.gate_d, a.up_d};
+template <int WT, int CT, int KS>
+__device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds,
+                                             MoeShared& sh) {
     f4 acc[2][CT];
-    auto stage = [&](int c0, int blocks) {
-        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
-            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
-            const uint16_t* x = a.x + (size_t)(sh.list[t0 + t] / a.top) * a.K + (c0 + b) * 32;
-            sh.stage[(b * 4 + s) * nt + t] = piece<WT>(*(const h4*)(x + run0<WT>(s)), *(const h4*)(x + run1<WT>(s)));
+    const StageX<WT> stage{a, sh.list + t0, nt};
+    const int tiles = a.I / 16, nb = a.K / 32;
+    // (a wave past the last tile computes that one and stores nothing)
+    const size_t row = (size_t)e * a.I + 16 * (tile < tiles ? tile : tiles - 1);
+    const Rows<WT> w[2] = {Rows<WT>(a.gate, row, nb), Rows<WT>(a.up, row, nb)};
+    const uint16_t* const wd[2] = {a.gate_d, a.up_d};
+    multiply<WT, 2, CT, KS>(w, wd, row, nb, stage, at, lds, sh, acc);
+    const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4;
+    if ((threadIdx.x >> 6) % KS || tile >= tiles) return;
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const int t = 16 * c + c16 < nt ? 16 * c + c16 : nt - 1, pair = sh.list[t0 + t];
+        const float gw = sh.g[t0 + t];
+        f4 h;
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float gt = acc[0][c][i];
+            h[i] = gw * (gt / (1.0f + __expf(-gt)) * acc[1][c][i]);
+            m = fmaxf(m, fabsf(h[i]) <= 3.4028235e38f ? fabsf(h[i]) : INFINITY);   // (a NaN counts as an infinity)
         }
-    };
-    multiply<WT, 2, CT>(w, wd, (size_t)e * a.I + i0, a.K / 32, nt, stage, sh, acc);
-    for (int i = threadIdx.x; i < 16 * nt; i += kWaves * 64) {
-        const int row = i & 15, t = i >> 4, pair = sh.list[t0 + t];
-        const float gt = summed<2, CT>(sh, 0, t, row), up = summed<2, CT>(sh, 1, t, row);
-        const float h = a.g[pair] * (gt / (1.0f + __expf(-gt)) * up);
-        a.h[(size_t)pair * a.I + i0 + row] = h;
-        // the tile's largest |h| (a NaN counts as an infinity)
-        float m = fabsf(h) <= 3.4028235e38f ? fabsf(h) : INFINITY;
-        m = fmaxf(m, dpp_f<0xB1>(m));
-        m = fmaxf(m, dpp_f<0x4E>(m));
-        m = fmaxf(m, dpp_f<0x141>(m));
-        m = fmaxf(m, dpp_f<0x140>(m));
-        if (row == 0) a.hmax[(size_t)pair * (a.I / 16) + i0 / 16] = m;
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (16 * c + c16 >= nt) continue;
+        *(f4*)(a.h + (size_t)pair * a.I + 16 * tile + 4 * g) = h;
+        if (g == 0) a.hmax[(size_t)pair * tiles + tile] = m;   // the tile's largest |h|
     }
 }
 
-template <int WT>
-__global__ __launch_bounds__(kWaves * 64) void moe_gate_up_kernel(MoeArgs a) {
+template <int WT, int KS, int CT>
+__global__ __launch_bounds__(kWaves * 64) void moe_gate_up_kernel(MoeArgs a, Layout at) {
+    extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeShared sh;
-    const int tiles = a.I / 16, i0 = (int)(blockIdx.x % tiles) * 16;
-    const int e = slot_expert(a, blockIdx.x / tiles, sh);
+    constexpr int TW = kWaves / KS;   // tiles of a workgroup
+    const int groups = (a.I / 16 + TW - 1) / TW;
+    const int tile = (int)(blockIdx.x % groups) * TW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / KS;
+    const int e = __builtin_amdgcn_readfirstlane(slot_expert(a, blockIdx.x / groups, sh));
     if (e < 0) return;
     const int count = sh.count;
-    for (int t0 = 0; t0 < count; t0 += 32) {
-        const int nt = count - t0 < 32 ? count - t0 : 32;
-        if (nt <= 16) gate_up_tile<WT, 1>(a, e, i0, t0, nt, sh);
-        else gate_up_tile<WT, 2>(a, e, i0, t0, nt, sh);
+    for (int t0 = 0; t0 < count; t0 += 16 * CT) {
+        const int nt = count - t0 < 16 * CT ? count - t0 : 16 * CT;
+        if (CT == 1 || nt <= 16) gate_up_tile<WT, 1, KS>(a, e, tile, t0, nt, at, lds, sh);
+        else gate_up_tile<WT, CT, KS>(a, e, tile, t0, nt, at, lds, sh);
         __syncthreads();
     }
 }
 
+// 2^-e with m 2^-e in [2^14, 2^15); 1 for zeros and the non-finite.
+__device__ __forceinline__ float scale_for(float m) {
+    return m > 0.0f && m < INFINITY ? ldexpf(1.0f, min(14 - ilogbf(m), 126)) : 1.0f;
+}
+
 // Down: 16 rows of one expert; the columns are the hi and lo parts of each
 // token's h, one after the other.
-template <int WT, int CT>
-__device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int n0, int t0, int nt, MoeShared& sh) {
-    const void* const w[1] = {a.down};
-    const uint16_t* const wd[1] = {a.down_d};
+template <int WT, int CT, int KS>
+__device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds, MoeShared& sh) {
     f4 acc[1][CT];
-    auto stage = [&](int c0, int blocks) {
-        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
-            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
-            const float* h = a.h + (size_t)sh.list[t0 + t] * a.I + (c0 + b) * 32;
-            const float f = sh.scale[t0 + t];
-            const f4 p = *(const f4*)(h + run0<WT>(s)) * f, q = *(const f4*)(h + run1<WT>(s)) * f;
-            f4 pl, ql;
+    const StageH<WT> stage{a, sh.list + t0, nt, sh.scale + t0};
+    const int tiles = a.K / 16, nb = a.I / 32;
+    const size_t row = (size_t)e * a.K + 16 * (tile < tiles ? tile : tiles - 1);
+    const Rows<WT> w[1] = {Rows<WT>(a.down, row, nb)};
+    const uint16_t* const wd[1] = {a.down_d};
+    multiply<WT, 1, CT, KS>(w, wd, row, nb, stage, at, lds, sh, acc);
+    const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4;
+    if ((threadIdx.x >> 6) % KS || tile >= tiles) return;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                pl[k] = p[k] - (float)(h16)p[k];
-                ql[k] = q[k] - (float)(h16)q[k];
-            }
-            h8* dst = sh.stage + (size_t)(b * 4 + s) * (2 * nt) + 2 * t;
-            dst[0] = piece<WT>(p, q);
-            dst[1] = piece<WT>(pl, ql);
-        }
-    };
-    multiply<WT, 1, CT>(w, wd, (size_t)e * a.K + n0, a.I / 32, 2 * nt, stage, sh, acc);
-    for (int i = threadIdx.x; i < 16 * nt; i += kWaves * 64) {
-        const int row = i & 15, t = i >> 4;
-        const float v = (summed<1, CT>(sh, 0, 2 * t, row) + summed<1, CT>(sh, 0, 2 * t + 1, row)) / sh.scale[t0 + t];
-        a.part[(size_t)sh.list[t0 + t] * a.K + n0 + row] = v;
+    for (int c = 0; c < CT; c++) {
+        const int t = 8 * c + (c16 >> 1);
+        f4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = acc[0][c][i] + dpp_f<0xB1>(acc[0][c][i]);   // hi + lo
+        if (t >= nt || (c16 & 1)) continue;
+        const float f = 1.0f / sh.scale[t0 + t];
+        *(f4*)(a.part + (size_t)sh.list[t0 + t] * a.K + 16 * tile + 4 * g) = v * f;
     }
 }
 
-template <int WT>
-__global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a) {
+template <int WT, int KS, int CT>
+__global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a, Layout at) {
+    extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeShared sh;
-    const int tiles = a.K / 16, n0 = (int)(blockIdx.x % tiles) * 16;
-    const int e = slot_expert(a, blockIdx.x / tiles, sh);
+    constexpr int TW = kWaves / KS;
+    const int groups = (a.K / 16 + TW - 1) / TW;
+    const int tile = (int)(blockIdx.x % groups) * TW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / KS;
+    const int e = __builtin_amdgcn_readfirstlane(slot_expert(a, blockIdx.x / groups, sh));
     if (e < 0) return;
     const int count = sh.count, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int t = wave; t < count; t += kWaves) {
@@ -406,81 +562,14 @@ __global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a) {
         float m = 0.0f;
         for (int i = lane; i < a.I / 16; i += 64) m = fmaxf(m, hm[i]);
         m = wave_max(m);
-        // 2^-e with m 2^-e in [2^14, 2^15); 1 for zeros and the non-finite
-        if (lane == 0) sh.scale[t] = m > 0.0f && m < INFINITY ? ldexpf(1.0f, min(14 - ilogbf(m), 126)) : 1.0f;
+        if (lane == 0) sh.scale[t] = scale_for(m);
     }
     __syncthreads();
-    for (int t0 = 0; t0 < count; t0 += 16) {
-        const int nt = count - t0 < 16 ? count - t0 : 16;
-        if (nt <= 8) down_tile<WT, 1>(a, e, n0, t0, nt, sh);
-        else down_tile<WT, 2>(a, e, n0, t0, nt, sh);
+    for (int t0 = 0; t0 < count; t0 += 8 * CT) {
+        const int nt = count - t0 < 8 * CT ? count - t0 : 8 * CT;
+        if (CT == 1 || nt <= 8) down_tile<WT, 1, KS>(a, e, tile, t0, nt, at, lds, sh);
+        else down_tile<WT, CT, KS>(a, e, tile, t0, nt, at, lds, sh);
         __syncthreads();
-    }
-}
-
-// Down for a single token: all its experts in one workgroup per 16 rows, so
-// that no sum is left over.  Sixteen waves share out the (expert, step) pairs;
-// the columns are hi and lo of h under one power of two.
-constexpr int kOneSteps = 64;   // steps of 4 blocks staged at a time (32 KB)
-template <int WT>
-__global__ __launch_bounds__(1024) void moe_down_one_kernel(MoeArgs a) {
-    __shared__ h8 stage[kOneSteps * 32];
-    __shared__ float red[16][2][16], most[16];
-    constexpr int PD = WT == TLHIP_F16 ? 1 : 2;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + 3) / 4, steps = a.top * per;
-    const int ids = a.ids[lane < a.top ? lane : 0];
-    auto load = [&](Weights<WT>& w, int n) {
-        const int t = n < steps ? n / per : 0, e = __builtin_amdgcn_readlane(ids, t);
-        // (past the last step: a step past the row's end, which loads nothing)
-        w.load(a.down, a.down_d, (size_t)e * a.K + n0 + c16, nb, n < steps ? n - t * per : per, g);
-    };
-    Weights<WT> ring[PD];
-#pragma unroll
-    for (int k = 0; k < PD; k++) load(ring[k], wave + 16 * k);
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < a.top * (a.I / 16); i += 1024) m = fmaxf(m, a.hmax[i]);
-    m = block_max1<16>(m, most);
-    const float scale = m > 0.0f && m < INFINITY ? ldexpf(1.0f, min(14 - ilogbf(m), 126)) : 1.0f;
-    f4 acc = {0, 0, 0, 0};
-    for (int s0 = 0; s0 < steps; s0 += kOneSteps) {
-        const int n1 = steps - s0 < kOneSteps ? steps - s0 : kOneSteps;
-        lds_barrier();
-        for (int i = threadIdx.x; i < n1 * 16; i += 1024) {
-            const int s = i & 3, b = i >> 2, n = s0 + (b >> 2), t = n / per, block = 4 * (n - t * per) + (b & 3);
-            f4 p = {0, 0, 0, 0}, q = p, pl, ql;
-            if (block < nb) {
-                const float* h = a.h + (size_t)t * a.I + block * 32;
-                p = *(const f4*)(h + run0<WT>(s)) * scale;
-                q = *(const f4*)(h + run1<WT>(s)) * scale;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                pl[k] = p[k] - (float)(h16)p[k];
-                ql[k] = q[k] - (float)(h16)q[k];
-            }
-            stage[2 * i] = piece<WT>(p, q);
-            stage[2 * i + 1] = piece<WT>(pl, ql);
-        }
-        lds_barrier();
-        for (int n = wave; n < n1; n += 16) {
-            const Weights<WT> cur = ring[0];
-#pragma unroll
-            for (int k = 1; k < PD; k++) ring[k - 1] = ring[k];
-            load(ring[PD - 1], s0 + n + 16 * PD);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const h8 x = stage[((4 * n + piece_block<WT>(j, g)) * 4 + piece_sub<WT>(j, g)) * 2 + (c16 & 1)];
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(cur.sub(j), x, acc, 0, 0, 0);
-            }
-        }
-    }
-    if (c16 < 2) *(f4*)&red[wave][c16][4 * g] = acc;
-    __syncthreads();
-    if (threadIdx.x < 16) {
-        float s = 0.0f;
-        for (int w = 0; w < 16; w++) s += red[w][0][threadIdx.x] + red[w][1][threadIdx.x];
-        a.y[n0 + threadIdx.x] = f2h(s / scale);
     }
 }
 
@@ -495,32 +584,153 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
     *(uint64_t*)y = (uint64_t)f2h(s[0]) | (uint64_t)f2h(s[1]) << 16 | (uint64_t)f2h(s[2]) << 32 | (uint64_t)f2h(s[3]) << 48;
 }
 
-}  // namespace
-
+// Down for a single token: all its experts in one workgroup per 16 rows, so
+// that no sum is left over.  Sixteen waves share out the (expert, slot) pairs;
+// the columns are hi and lo of h under one power of two, all of them in LDS at
+// once: blocks of expert t from t * per slots on.
+constexpr int kOneWaves = 16;
 template <int WT>
-static void launch_gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    moe_gate_up_kernel<WT><<<slots * (a.I / 16), kWaves * 64, 0, s>>>(a);
+__host__ __device__ inline Layout layout_one(int nb, int top) {
+    const int per = (nb + Slot<WT>::BLOCKS - 1) / Slot<WT>::BLOCKS;
+    Layout l;
+    l.column_bytes = top * per * Slot<WT>::BLOCKS * 128;
+    l.ring_at = l.column_bytes;
+    l.scales_at = l.ring_at + kOneWaves * kRing * Slot<WT>::BYTES;
+    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : top * 32 * nb);
+    return l;
 }
 template <int WT>
-static void launch_down(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    if (a.M == 1) {
-        moe_down_one_kernel<WT><<<a.K / 16, 1024, 0, s>>>(a);
-        return;
+__global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a, Layout at) {
+    using S = Slot<WT>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ float red[kOneWaves][2][16], most[kOneWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + S::BLOCKS - 1) / S::BLOCKS, slots = a.top * per;
+    h8* cols = (h8*)lds;
+    const uint8_t* ring = lds + at.ring_at + wave * (kRing * S::BYTES);
+    const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(ring));
+    uint16_t* scales = (uint16_t*)(lds + at.scales_at);
+    const int ids = a.ids[lane < a.top ? lane : 0];
+    auto copy = [&](int n, int k) {
+        const int t = n / per, e = __builtin_amdgcn_readlane(ids, t);
+        Rows<WT>(a.down, (size_t)e * a.K + n0, nb).copy(n - t * per, ring_lds + k * S::BYTES);
+    };
+    int next = wave, place = 0;
+#pragma unroll
+    for (int k = 0; k < kRing; k++, next += kOneWaves)
+        if (next < slots) copy(next, k);
+    if constexpr (WT != TLHIP_F16)
+        for (int t = 0; t < a.top; t++)
+            copy_scales(scales + t * 16 * nb, a.down_d, (size_t)__builtin_amdgcn_readlane(ids, t) * a.K + n0, nb, threadIdx.x, kOneWaves * 64);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < a.top * (a.I / 16); i += kOneWaves * 64) m = fmaxf(m, a.hmax[i]);
+    m = block_max1<kOneWaves>(m, most);
+    const float scale = scale_for(m);
+    for (int i = threadIdx.x; i < slots * S::BLOCKS * 4; i += kOneWaves * 64) {
+        const int s = i & 3, t = (i >> 2) / (per * S::BLOCKS), b = (i >> 2) - t * (per * S::BLOCKS);
+        f4 p = {0, 0, 0, 0}, q = p;
+        if (b < nb) {
+            const float* h = a.h + (size_t)t * a.I + b * 32;
+            p = *(const f4*)(h + run0<WT>(s)) * scale;
+            q = *(const f4*)(h + run1<WT>(s)) * scale;
+        }
+        cols[2 * i] = piece<WT>(p, q);
+        cols[2 * i + 1] = piece<WT>(low_part(p), low_part(q));
     }
-    moe_down_kernel<WT><<<slots * (a.K / 16), kWaves * 64, 0, s>>>(a);
-    moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
+    lds_barrier();
+    f4 acc = {0, 0, 0, 0};
+    for (int n = wave; n < slots; n += kOneWaves) {
+        if (next > n + (kRing - 1) * kOneWaves) sk_wait_vm<(kRing - 1) * S::COPIES>();
+        else sk_wait_vm<0>();
+        const int t = n / per;
+        Weights<WT> w[S::STEPS];
+#pragma unroll
+        for (int u = 0; u < S::STEPS; u++)
+            w[u].read(ring + place * S::BYTES, scales + t * 16 * nb, c16, nb, (n - t * per) * S::BLOCKS, u, g);
+        if (next < slots) {
+            lds_reads_done();
+            copy(next, place);
+            next += kOneWaves;
+        }
+        place = place + 1 == kRing ? 0 : place + 1;
+#pragma unroll
+        for (int u = 0; u < S::STEPS; u++) {
+            h8 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[j] = cols[((n * S::BLOCKS + 4 * u + piece_block<WT>(j, g)) * 4 + piece_sub<WT>(j, g)) * 2 + (c16 & 1)];
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[u].sub(j), x[j], acc, 0, 0, 0);
+        }
+    }
+    if (c16 < 2) *(f4*)&red[wave][c16][4 * g] = acc;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float s = 0.0f;
+        for (int w = 0; w < kOneWaves; w++) s += red[w][0][threadIdx.x] + red[w][1][threadIdx.x];
+        a.y[n0 + threadIdx.x] = f2h(s / scale);
+    }
 }
+
+// Dynamic LDS beside MoeShared, of 160 KB.  Rows of kMoeMaxRow fit with four
+// waves to a tile: at most 64 KB of columns, 64 KB of rings and 64 bytes of
+// scales per block (f16: none).
+constexpr int kLdsDynamic = 140 << 10;
+static_assert(kLdsDynamic + sizeof(MoeShared) <= 160 << 10, "LDS of a CU");
+static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "Q4_0 rows fit");
+static_assert((32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
+
+// A tile of 16 rows goes to one wave where there are tiles enough to keep
+// eight waves on every CU (and LDS holds four tiles' scales), else to four that
+// share out k.  Up to 16 (down: 8) tokens, no expert has more columns than one
+// B operand holds.
+constexpr int64_t kTilesEnough = 2048;
+template <int WT, int KS>
+tlhip_status gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    const unsigned grid = slots * ((a.I / 16 + kWaves / KS - 1) / (kWaves / KS));
+    const Layout at = layout<WT, 2, KS>(a.K / 32, a.M < 32 ? a.M : 32);
+    if (a.M <= 16) moe_gate_up_kernel<WT, KS, 1><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    else moe_gate_up_kernel<WT, KS, 2><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    return TLHIP_OK;
+}
+template <int WT, int KS>
+tlhip_status down(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    const unsigned grid = slots * ((a.K / 16 + kWaves / KS - 1) / (kWaves / KS));
+    const Layout at = layout<WT, 1, KS>(a.I / 32, a.M < 16 ? 2 * a.M : 32);
+    if (a.M <= 8) moe_down_kernel<WT, KS, 1><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    else moe_down_kernel<WT, KS, 2><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
+    return TLHIP_OK;
+}
+template <int WT>
+tlhip_status gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    if ((int64_t)slots * (a.I / 16) >= kTilesEnough && layout<WT, 2, 1>(a.K / 32, 32).bytes <= kLdsDynamic) return gate_up<WT, 1>(s, a, slots);
+    return gate_up<WT, 4>(s, a, slots);
+}
+template <int WT>
+tlhip_status down(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    if (a.M == 1) {
+        const Layout at = layout_one<WT>(a.I / 32, a.top);
+        if (at.bytes <= kLdsDynamic) {
+            moe_down_one_kernel<WT><<<a.K / 16, kOneWaves * 64, at.bytes, s>>>(a, at);
+            return TLHIP_OK;
+        }
+    }
+    if ((int64_t)slots * (a.K / 16) >= kTilesEnough && layout<WT, 1, 1>(a.I / 32, 32).bytes <= kLdsDynamic) return down<WT, 1>(s, a, slots);
+    return down<WT, 4>(s, a, slots);
+}
+
+}  // namespace
 
 tlhip_status launch_moe(hipStream_t s, const MoeArgs& a) {
     moe_router_kernel<<<a.M, 1024, 0, s>>>(a);
     const unsigned slots = a.M * a.top < a.E ? a.M * a.top : a.E;
-    if (a.wt_gu == TLHIP_F16) launch_gate_up<TLHIP_F16>(s, a, slots);
-    else if (a.wt_gu == TLHIP_Q4_0) launch_gate_up<TLHIP_Q4_0>(s, a, slots);
-    else launch_gate_up<TLHIP_Q8_0>(s, a, slots);
-    if (a.wt_down == TLHIP_F16) launch_down<TLHIP_F16>(s, a, slots);
-    else if (a.wt_down == TLHIP_Q4_0) launch_down<TLHIP_Q4_0>(s, a, slots);
-    else launch_down<TLHIP_Q8_0>(s, a, slots);
-    return TLHIP_OK;
+    if (a.wt_gu == TLHIP_F16) TLHIP_TRY(gate_up<TLHIP_F16>(s, a, slots));
+    else if (a.wt_gu == TLHIP_Q4_0) TLHIP_TRY(gate_up<TLHIP_Q4_0>(s, a, slots));
+    else TLHIP_TRY(gate_up<TLHIP_Q8_0>(s, a, slots));
+    if (a.wt_down == TLHIP_F16) return down<TLHIP_F16>(s, a, slots);
+    if (a.wt_down == TLHIP_Q4_0) return down<TLHIP_Q4_0>(s, a, slots);
+    return down<TLHIP_Q8_0>(s, a, slots);
 }
 
 }  // namespace tlhip

@@ -50,8 +50,9 @@ extern "C" tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor ro
     if (Iu != I || Kd != K || gate->dtype != up->dtype)
         return fail(TLHIP_ERR_SHAPE_MISMATCH, "moe: gate %s, up %s and down %s (gate and up of one dtype)",
                     shape_str(gate).c_str(), shape_str(up).c_str(), shape_str(down).c_str());
-    if (K < 32 || I < 32 || K % 32 || I % 32 || E * K > INT32_MAX || E * I > INT32_MAX)
-        return fail(TLHIP_ERR_INVALID_DIMENSION, "moe: rows of %lld and %lld (multiples of 32)", (long long)K, (long long)I);
+    if (K < 32 || I < 32 || K % 32 || I % 32 || K > kMoeMaxRow || I > kMoeMaxRow)
+        return fail(TLHIP_ERR_INVALID_DIMENSION, "moe: rows of %lld and %lld (multiples of 32 up to %d)", (long long)K, (long long)I,
+                    kMoeMaxRow);
     if (M == 0) return TLHIP_OK;
     const int64_t slab = M < kSlab ? M : kSlab;
     // ids, g, h, hmax, part: one after another
