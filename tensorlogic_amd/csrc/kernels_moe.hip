@@ -37,9 +37,12 @@ namespace tlhip {
 namespace {
 
 constexpr int kWaves = 4;                  // of a workgroup of the products
-constexpr int kColumnBytes = 32 << 10;     // columns staged in LDS at a time (or one round of slots, if that is more)
 constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
-constexpr int kRing = 2;                   // slots of weights a wave has in flight
+// By the matrices of a product (gate and up: 2, down: 1): slots of weights that
+// a wave has in flight, and the columns staged in LDS at a time (or one round of
+// slots, if that is more).  Both leave room for two workgroups on a CU.
+constexpr int ring_slots(int nr) { return nr == 2 ? 2 : 4; }
+constexpr int column_budget(int nr) { return (nr == 2 ? 24 : 40) << 10; }
 
 // ---------------------------------------------------------------------------
 // router
@@ -249,11 +252,16 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 // This wave's LDS reads are done (their memory may be copied over).
 __device__ __forceinline__ void lds_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The scales of 16 rows (nb of them each, which lie together) to LDS, by all
-// threads of `threads`.
-__device__ __forceinline__ void copy_scales(uint16_t* dst, const uint16_t* d, size_t row, int nb, int thread, int threads) {
-    const u4* src = (const u4*)(d + row * nb);   // (16 nb values from a multiple of 16: 32-byte aligned)
-    for (int i = thread; i < 2 * nb; i += threads) ((u4*)dst)[i] = src[i];
+// The scales of 16 rows (nb of each row, which lie together: 2 nb pieces of 16
+// bytes) to LDS, copies part, part + parts, ... of 1 KB.  The last copy repeats
+// the last piece: room in LDS is in whole KB.
+__host__ __device__ constexpr int scale_bytes(int nb) { return (32 * nb + 1023) / 1024 * 1024; }
+__device__ __forceinline__ void copy_scales(uint32_t lds, const uint16_t* d, size_t row, int nb, int part, int parts) {
+    const __amdgpu_buffer_rsrc_t r = sk_rsrc(d + row * nb, 32u * nb);
+    for (int i = part; i * 64 < 2 * nb; i += parts) {
+        const int at = i * 64 + (int)(threadIdx.x & 63);
+        sk_dma<16>(r, lds + i * 1024, (at < 2 * nb ? at : 2 * nb - 1) * 16);
+    }
 }
 
 // What a workgroup holds in LDS before its dynamic part, which is: columns,
@@ -262,7 +270,6 @@ struct MoeShared {
     int list[kTokens];      // the expert's (token, choice) pairs
     float g[kTokens];       // their weights
     float scale[kTokens];   // down: 2^-e of each
-    f4 red[kWaves * 4 * 64];
     int count;
 };
 
@@ -287,15 +294,6 @@ __device__ __forceinline__ void find_tokens(const MoeArgs& a, int e, MoeShared& 
 // nothing to do.  With fewer (token, choice) pairs than experts a slot is a
 // pair, and only the first pair of an expert works on it; else an expert.
 __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared& sh) {
-    if (a.M == 1 && a.top < a.E) {
-        if (threadIdx.x == 0) {
-            sh.list[0] = slot;
-            sh.g[0] = a.g[slot];
-            sh.count = 1;
-        }
-        __syncthreads();
-        return a.ids[slot];
-    }
     const bool by_pair = a.M * a.top < a.E;
     const int e = by_pair ? a.ids[slot] : slot;
     if (threadIdx.x < 64) find_tokens(a, e, sh);
@@ -303,33 +301,45 @@ __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared
     return by_pair && sh.list[0] != slot ? -1 : e;
 }
 
-// The columns of gate and up: x of the tokens list[0 .. nt).  Block b, piece s
-// of token t is 16 bytes at (4 b + s) * ncol + t; past the row's nb blocks zeros.
-template <int WT>
-struct StageX {
-    const MoeArgs& a;
-    const int* list;
-    int nt;
-    __device__ __forceinline__ int ncol() const { return nt; }
-    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
-        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
-            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
-            h8 v = {};
-            if (c0 + b < nb) {
-                const uint16_t* x = a.x + (size_t)(list[t] / a.top) * a.K + (c0 + b) * 32;
-                v = piece<WT>(*(const h4*)(x + run0<WT>(s)), *(const h4*)(x + run1<WT>(s)));
-            }
-            cols[(b * 4 + s) * nt + t] = v;
-        }
-    }
-};
-// Those of down: hi and lo of each token's h 2^-e.
+// The columns of a product.  Column c of piece s of block b is 16 bytes at
+// (4 b + s) * ncol + c; past the row's nb blocks they are zeros.  A thread
+// loads four pieces before it stores any.
 __device__ __forceinline__ f4 low_part(const f4& p) {
     f4 r;
 #pragma unroll
     for (int k = 0; k < 4; k++) r[k] = p[k] - (float)(h16)p[k];
     return r;
 }
+// Gate and up: x of the tokens list[0 .. nt), or of the only token.
+template <int WT, bool ONE>
+struct StageX {
+    const MoeArgs& a;
+    const int* list;
+    int nt;
+    __device__ __forceinline__ int ncol() const { return nt; }
+    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
+        const uint32_t by_nt = 0xFFFFFFFFu / nt + 1;   // i / nt = umulhi(i, by_nt): i nt < 2^32
+        for (int i0 = threadIdx.x; i0 < blocks * 4 * nt; i0 += 4 * kWaves * 64) {
+            h4 p[4], q[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = i0 + k * kWaves * 64, bs = nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * nt, b = c0 + (bs >> 2);
+                p[k] = q[k] = h4{};
+                if (i < blocks * 4 * nt && b < nb) {
+                    const uint16_t* x = a.x + (ONE ? 0 : (size_t)(list[t] / a.top) * a.K) + b * 32;
+                    p[k] = *(const h4*)(x + run0<WT>(bs & 3));
+                    q[k] = *(const h4*)(x + run1<WT>(bs & 3));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = i0 + k * kWaves * 64;
+                if (i < blocks * 4 * nt) cols[i] = piece<WT>(p[k], q[k]);
+            }
+        }
+    }
+};
+// Down: hi and lo of each token's h 2^-e, one after the other.
 template <int WT>
 struct StageH {
     const MoeArgs& a;
@@ -338,17 +348,26 @@ struct StageH {
     const float* scale;
     __device__ __forceinline__ int ncol() const { return 2 * nt; }
     __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
-        for (int i = threadIdx.x; i < blocks * 4 * nt; i += kWaves * 64) {
-            const int s = i & 3, b = (i >> 2) % blocks, t = (i >> 2) / blocks;
-            f4 p = {0, 0, 0, 0}, q = p;
-            if (c0 + b < nb) {
-                const float* h = a.h + (size_t)list[t] * a.I + (c0 + b) * 32;
-                p = *(const f4*)(h + run0<WT>(s)) * scale[t];
-                q = *(const f4*)(h + run1<WT>(s)) * scale[t];
+        const uint32_t by_nt = 0xFFFFFFFFu / nt + 1;
+        for (int i0 = threadIdx.x; i0 < blocks * 4 * nt; i0 += 4 * kWaves * 64) {
+            f4 p[4], q[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = i0 + k * kWaves * 64, bs = nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * nt, b = c0 + (bs >> 2);
+                p[k] = q[k] = f4{0, 0, 0, 0};
+                if (i < blocks * 4 * nt && b < nb) {
+                    const float* h = a.h + (size_t)list[t] * a.I + b * 32;
+                    p[k] = *(const f4*)(h + run0<WT>(bs & 3)) * scale[t];
+                    q[k] = *(const f4*)(h + run1<WT>(bs & 3)) * scale[t];
+                }
             }
-            h8* dst = cols + (b * 4 + s) * (2 * nt) + 2 * t;
-            dst[0] = piece<WT>(p, q);
-            dst[1] = piece<WT>(low_part(p), low_part(q));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = i0 + k * kWaves * 64;
+                if (i >= blocks * 4 * nt) continue;
+                cols[2 * i] = piece<WT>(p[k], q[k]);
+                cols[2 * i + 1] = piece<WT>(low_part(p[k]), low_part(q[k]));
+            }
         }
     }
 };
@@ -358,35 +377,37 @@ struct StageH {
 struct Layout {
     int column_bytes, ring_at, scales_at, bytes;
 };
+constexpr int kRedBytes = kWaves * 4 * 64 * 16;   // the waves' sums, in place of columns and ring at the end
 template <int WT, int NR, int KS>
 __host__ __device__ inline Layout layout(int nb, int max_cols) {
     constexpr int round = Slot<WT>::BLOCKS * KS;
     Layout l;
     const int whole = (nb + round - 1) / round * round * 64 * max_cols, least = round * 64 * max_cols;
-    l.column_bytes = whole < kColumnBytes ? whole : kColumnBytes > least ? kColumnBytes : least;
+    l.column_bytes = whole < column_budget(NR) ? whole : column_budget(NR) > least ? column_budget(NR) : least;
     l.ring_at = l.column_bytes;
-    l.scales_at = l.ring_at + kWaves * NR * kRing * Slot<WT>::BYTES;
-    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : kWaves / KS * NR * 32 * nb);
+    l.scales_at = l.ring_at + kWaves * NR * ring_slots(NR) * Slot<WT>::BYTES;
+    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : kWaves / KS * NR * scale_bytes(nb));
+    if (KS > 1 && l.bytes < kRedBytes) l.bytes = kRedBytes;
     return l;
 }
 
 // acc[r][c] = W_r (16 rows, nb blocks) times the CT * 16 columns that stage()
 // lays out chunk by chunk, k shared out over KS waves.  Complete in the first
 // of them: lane (c16, g) has rows 4g .. 4g + 3 of column c16.
-template <int WT, int NR, int CT, int KS, typename STAGE>
+template <int WT, int NR, int CT, int KS, bool ONE, typename STAGE>
 __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t* const (&wd)[NR], size_t row, int nb, const STAGE& stage,
                                          const Layout& at, uint8_t* lds, MoeShared& sh, f4 (&acc)[NR][CT]) {
     using S = Slot<WT>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS;
     const int c16 = lane & 15, g = lane >> 4, ncol = stage.ncol();
-    constexpr int ROUND = S::BLOCKS * KS;
+    constexpr int ROUND = S::BLOCKS * KS, kRing = ring_slots(NR);
     int chunk = at.column_bytes / (64 * ncol) / ROUND * ROUND;   // blocks of a chunk: whole rounds of the KS waves' slots
     const int all = (nb + ROUND - 1) / ROUND * ROUND;
     if (chunk > all) chunk = all;
     h8* cols = (h8*)lds;
     const uint8_t* ring = lds + at.ring_at + wave * (NR * kRing * S::BYTES);
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(ring));
-    uint16_t* scales = (uint16_t*)(lds + at.scales_at) + wave / KS * (NR * 16 * nb);
+    const uint8_t* scales = lds + at.scales_at + wave / KS * (NR * scale_bytes(nb));
     int col[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) col[c] = 16 * c + c16 < ncol ? 16 * c + c16 : ncol - 1;
@@ -399,17 +420,29 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
 #pragma unroll
         for (int r = 0; r < NR; r++) w[r].copy(n, ring_lds + (k * NR + r) * S::BYTES);
     };
+    // One token's columns do not wait for the router's choice, which the copies
+    // do: they go first, and copies return in order.  Else the copies go first.
+    if constexpr (ONE) stage(cols, 0, chunk, nb);
+    if constexpr (WT != TLHIP_F16) {
+        const uint32_t scales_lds = __builtin_amdgcn_readfirstlane(lds_address(scales));
+#pragma unroll
+        for (int r = 0; r < NR; r++) copy_scales(scales_lds + r * scale_bytes(nb), wd[r], row, nb, part, KS);
+    }
     int next = part, place = 0;   // the next slot to copy
 #pragma unroll
     for (int k = 0; k < kRing; k++, next += KS)
         if (next < slots) copy(next, k);
-    if constexpr (WT != TLHIP_F16)
-#pragma unroll
-        for (int r = 0; r < NR; r++) copy_scales(scales + r * 16 * nb, wd[r], row, nb, threadIdx.x % (KS * 64), KS * 64);
+    if constexpr (ONE) {   // the scales have landed
+        if (next <= slots - 1 + KS) sk_wait_vm<kRing * NR * S::COPIES>();
+        else sk_wait_vm<0>();
+    }
     for (int c0 = 0; c0 < all; c0 += chunk) {
         const int blocks = all - c0 < chunk ? all - c0 : chunk;
-        lds_barrier();
-        stage(cols, c0, blocks, nb);
+        if (!ONE || c0) {   // (its loads are waited for, so the scales have landed)
+            lds_barrier();
+            stage(cols, c0, blocks, nb);
+            sk_wait_vm<0>();
+        }
         lds_barrier();
         const int end = min((c0 + blocks) / S::BLOCKS, slots);
         for (int n = c0 / S::BLOCKS + part; n < end; n += KS) {
@@ -422,7 +455,7 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
 #pragma unroll
             for (int r = 0; r < NR; r++)
 #pragma unroll
-                for (int u = 0; u < S::STEPS; u++) a[r][u].read(slot + r * S::BYTES, scales + r * 16 * nb, c16, nb, n * S::BLOCKS, u, g);
+                for (int u = 0; u < S::STEPS; u++) a[r][u].read(slot + r * S::BYTES, (const uint16_t*)(scales + r * scale_bytes(nb)), c16, nb, n * S::BLOCKS, u, g);
             if (next < slots) {
                 lds_reads_done();
                 copy(next, place);
@@ -450,10 +483,12 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
         }
     }
     if constexpr (KS > 1) {
+        f4* red = (f4*)lds;
+        lds_barrier();
 #pragma unroll
         for (int r = 0; r < NR; r++)
 #pragma unroll
-            for (int c = 0; c < CT; c++) sh.red[((wave * NR + r) * CT + c) * 64 + lane] = acc[r][c];
+            for (int c = 0; c < CT; c++) red[((wave * NR + r) * CT + c) * 64 + lane] = acc[r][c];
         lds_barrier();
         if (part == 0)
 #pragma unroll
@@ -461,28 +496,28 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
 #pragma unroll
                 for (int r = 0; r < NR; r++)
 #pragma unroll
-                    for (int c = 0; c < CT; c++) acc[r][c] += sh.red[(((wave + k) * NR + r) * CT + c) * 64 + lane];
+                    for (int c = 0; c < CT; c++) acc[r][c] += red[(((wave + k) * NR + r) * CT + c) * 64 + lane];
     }
 }
 
 // Gate and up of 16 rows of one expert, for tokens list[t0 .. t0 + nt).
-template <int WT, int CT, int KS>
+template <int WT, int CT, int KS, bool ONE>
 __device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds,
-                                             MoeShared& sh) {
+                                             MoeShared& sh, int one_pair = 0) {
     f4 acc[2][CT];
-    const StageX<WT> stage{a, sh.list + t0, nt};
+    const StageX<WT, ONE> stage{a, sh.list + t0, nt};
     const int tiles = a.I / 16, nb = a.K / 32;
     // (a wave past the last tile computes that one and stores nothing)
     const size_t row = (size_t)e * a.I + 16 * (tile < tiles ? tile : tiles - 1);
     const Rows<WT> w[2] = {Rows<WT>(a.gate, row, nb), Rows<WT>(a.up, row, nb)};
     const uint16_t* const wd[2] = {a.gate_d, a.up_d};
-    multiply<WT, 2, CT, KS>(w, wd, row, nb, stage, at, lds, sh, acc);
+    multiply<WT, 2, CT, KS, ONE>(w, wd, row, nb, stage, at, lds, sh, acc);
     const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4;
     if ((threadIdx.x >> 6) % KS || tile >= tiles) return;
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        const int t = 16 * c + c16 < nt ? 16 * c + c16 : nt - 1, pair = sh.list[t0 + t];
-        const float gw = sh.g[t0 + t];
+        const int t = 16 * c + c16 < nt ? 16 * c + c16 : nt - 1, pair = ONE ? one_pair : sh.list[t0 + t];
+        const float gw = ONE ? a.g[one_pair] : sh.g[t0 + t];
         f4 h;
         float m = 0.0f;
 #pragma unroll
@@ -499,20 +534,25 @@ __device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int tile, 
     }
 }
 
-template <int WT, int KS, int CT>
+template <int WT, int KS, int CT, bool ONE>
 __global__ __launch_bounds__(kWaves * 64) void moe_gate_up_kernel(MoeArgs a, Layout at) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeShared sh;
     constexpr int TW = kWaves / KS;   // tiles of a workgroup
     const int groups = (a.I / 16 + TW - 1) / TW;
     const int tile = (int)(blockIdx.x % groups) * TW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / KS;
-    const int e = __builtin_amdgcn_readfirstlane(slot_expert(a, blockIdx.x / groups, sh));
+    const int slot = blockIdx.x / groups;
+    if constexpr (ONE) {   // a slot is one of the token's choices, each of another expert
+        gate_up_tile<WT, 1, KS, true>(a, a.ids[slot], tile, 0, 1, at, lds, sh, slot);
+        return;
+    }
+    const int e = __builtin_amdgcn_readfirstlane(slot_expert(a, slot, sh));
     if (e < 0) return;
     const int count = sh.count;
     for (int t0 = 0; t0 < count; t0 += 16 * CT) {
         const int nt = count - t0 < 16 * CT ? count - t0 : 16 * CT;
-        if (CT == 1 || nt <= 16) gate_up_tile<WT, 1, KS>(a, e, tile, t0, nt, at, lds, sh);
-        else gate_up_tile<WT, CT, KS>(a, e, tile, t0, nt, at, lds, sh);
+        if (CT == 1 || nt <= 16) gate_up_tile<WT, 1, KS, ONE>(a, e, tile, t0, nt, at, lds, sh);
+        else gate_up_tile<WT, CT, KS, ONE>(a, e, tile, t0, nt, at, lds, sh);
         __syncthreads();
     }
 }
@@ -532,7 +572,7 @@ __device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int tile, int
     const size_t row = (size_t)e * a.K + 16 * (tile < tiles ? tile : tiles - 1);
     const Rows<WT> w[1] = {Rows<WT>(a.down, row, nb)};
     const uint16_t* const wd[1] = {a.down_d};
-    multiply<WT, 1, CT, KS>(w, wd, row, nb, stage, at, lds, sh, acc);
+    multiply<WT, 1, CT, KS, false>(w, wd, row, nb, stage, at, lds, sh, acc);
     const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4;
     if ((threadIdx.x >> 6) % KS || tile >= tiles) return;
 #pragma unroll
@@ -588,15 +628,15 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 // that no sum is left over.  Sixteen waves share out the (expert, slot) pairs;
 // the columns are hi and lo of h under one power of two, all of them in LDS at
 // once: blocks of expert t from t * per slots on.
-constexpr int kOneWaves = 16;
+constexpr int kOneWaves = 16, kOneRing = 2, kOnePieces = 2;
 template <int WT>
 __host__ __device__ inline Layout layout_one(int nb, int top) {
     const int per = (nb + Slot<WT>::BLOCKS - 1) / Slot<WT>::BLOCKS;
     Layout l;
     l.column_bytes = top * per * Slot<WT>::BLOCKS * 128;
     l.ring_at = l.column_bytes;
-    l.scales_at = l.ring_at + kOneWaves * kRing * Slot<WT>::BYTES;
-    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : top * 32 * nb);
+    l.scales_at = l.ring_at + kOneWaves * kOneRing * Slot<WT>::BYTES;
+    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : top * scale_bytes(nb));
     return l;
 }
 template <int WT>
@@ -607,52 +647,79 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + S::BLOCKS - 1) / S::BLOCKS, slots = a.top * per;
     h8* cols = (h8*)lds;
-    const uint8_t* ring = lds + at.ring_at + wave * (kRing * S::BYTES);
+    const uint8_t* ring = lds + at.ring_at + wave * (kOneRing * S::BYTES);
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(ring));
-    uint16_t* scales = (uint16_t*)(lds + at.scales_at);
+    const uint8_t* scales = lds + at.scales_at;
     const int ids = a.ids[lane < a.top ? lane : 0];
     auto copy = [&](int n, int k) {
         const int t = n / per, e = __builtin_amdgcn_readlane(ids, t);
         Rows<WT>(a.down, (size_t)e * a.K + n0, nb).copy(n - t * per, ring_lds + k * S::BYTES);
     };
-    int next = wave, place = 0;
+    // h and its largest value do not wait for the experts' numbers, which the
+    // copies do: they go first, and loads return in order
+    f4 p[kOnePieces], q[kOnePieces];
+    auto fetch = [&](int i0) {
 #pragma unroll
-    for (int k = 0; k < kRing; k++, next += kOneWaves)
-        if (next < slots) copy(next, k);
-    if constexpr (WT != TLHIP_F16)
-        for (int t = 0; t < a.top; t++)
-            copy_scales(scales + t * 16 * nb, a.down_d, (size_t)__builtin_amdgcn_readlane(ids, t) * a.K + n0, nb, threadIdx.x, kOneWaves * 64);
+        for (int k = 0; k < kOnePieces; k++) {
+            const int i = i0 + k * kOneWaves * 64, s = i & 3, t = (i >> 2) / (per * S::BLOCKS), b = (i >> 2) - t * (per * S::BLOCKS);
+            p[k] = q[k] = f4{0, 0, 0, 0};
+            if (i < slots * S::BLOCKS * 4 && b < nb) {
+                const float* h = a.h + (size_t)t * a.I + b * 32;
+                p[k] = *(const f4*)(h + run0<WT>(s));
+                q[k] = *(const f4*)(h + run1<WT>(s));
+            }
+        }
+    };
+    fetch(threadIdx.x);
     float m = 0.0f;
     for (int i = threadIdx.x; i < a.top * (a.I / 16); i += kOneWaves * 64) m = fmaxf(m, a.hmax[i]);
-    m = block_max1<kOneWaves>(m, most);
-    const float scale = scale_for(m);
-    for (int i = threadIdx.x; i < slots * S::BLOCKS * 4; i += kOneWaves * 64) {
-        const int s = i & 3, t = (i >> 2) / (per * S::BLOCKS), b = (i >> 2) - t * (per * S::BLOCKS);
-        f4 p = {0, 0, 0, 0}, q = p;
-        if (b < nb) {
-            const float* h = a.h + (size_t)t * a.I + b * 32;
-            p = *(const f4*)(h + run0<WT>(s)) * scale;
-            q = *(const f4*)(h + run1<WT>(s)) * scale;
-        }
-        cols[2 * i] = piece<WT>(p, q);
-        cols[2 * i + 1] = piece<WT>(low_part(p), low_part(q));
+    m = wave_max(m);
+    if (lane == 0) most[wave] = m;
+    if constexpr (WT != TLHIP_F16) {
+        const uint32_t scales_lds = __builtin_amdgcn_readfirstlane(lds_address(scales));
+        for (int t = 0; t < a.top; t++)
+            copy_scales(scales_lds + t * scale_bytes(nb), a.down_d, (size_t)__builtin_amdgcn_readlane(ids, t) * a.K + n0, nb, wave, kOneWaves);
     }
+    int next = wave, place = 0;
+#pragma unroll
+    for (int k = 0; k < kOneRing; k++, next += kOneWaves)
+        if (next < slots) copy(next, k);
+    lds_barrier();
+    m = most[0];
+#pragma unroll
+    for (int k = 1; k < kOneWaves; k++) m = fmaxf(m, most[k]);
+    const float scale = scale_for(m);
+    for (int i0 = threadIdx.x; i0 < slots * S::BLOCKS * 4; i0 += kOnePieces * kOneWaves * 64) {
+        if (i0 != (int)threadIdx.x) fetch(i0);
+#pragma unroll
+        for (int k = 0; k < kOnePieces; k++) {
+            const int i = i0 + k * kOneWaves * 64;
+            if (i >= slots * S::BLOCKS * 4) continue;
+            p[k] *= scale;
+            q[k] *= scale;
+            cols[2 * i] = piece<WT>(p[k], q[k]);
+            cols[2 * i + 1] = piece<WT>(low_part(p[k]), low_part(q[k]));
+        }
+    }
+    // the scales have landed (as many copies as the wave's slots came after them)
+    if (next <= slots - 1 + kOneWaves) sk_wait_vm<kOneRing * S::COPIES>();
+    else sk_wait_vm<0>();
     lds_barrier();
     f4 acc = {0, 0, 0, 0};
     for (int n = wave; n < slots; n += kOneWaves) {
-        if (next > n + (kRing - 1) * kOneWaves) sk_wait_vm<(kRing - 1) * S::COPIES>();
+        if (next > n + (kOneRing - 1) * kOneWaves) sk_wait_vm<(kOneRing - 1) * S::COPIES>();
         else sk_wait_vm<0>();
         const int t = n / per;
         Weights<WT> w[S::STEPS];
 #pragma unroll
         for (int u = 0; u < S::STEPS; u++)
-            w[u].read(ring + place * S::BYTES, scales + t * 16 * nb, c16, nb, (n - t * per) * S::BLOCKS, u, g);
+            w[u].read(ring + place * S::BYTES, (const uint16_t*)(scales + t * scale_bytes(nb)), c16, nb, (n - t * per) * S::BLOCKS, u, g);
         if (next < slots) {
             lds_reads_done();
             copy(next, place);
             next += kOneWaves;
         }
-        place = place + 1 == kRing ? 0 : place + 1;
+        place = place + 1 == kOneRing ? 0 : place + 1;
 #pragma unroll
         for (int u = 0; u < S::STEPS; u++) {
             h8 x[4];
@@ -675,49 +742,59 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
 // Dynamic LDS beside MoeShared, of 160 KB.  Rows of kMoeMaxRow fit with four
 // waves to a tile: at most 64 KB of columns, 64 KB of rings and 64 bytes of
 // scales per block (f16: none).
-constexpr int kLdsDynamic = 140 << 10;
+constexpr int kLdsDynamic = 156 << 10;
 static_assert(kLdsDynamic + sizeof(MoeShared) <= 160 << 10, "LDS of a CU");
-static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "Q4_0 rows fit");
-static_assert((32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
+static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "rows of a Q type fit");
+static_assert((40 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
 
-// A tile of 16 rows goes to one wave where there are tiles enough to keep
-// eight waves on every CU (and LDS holds four tiles' scales), else to four that
-// share out k.  Up to 16 (down: 8) tokens, no expert has more columns than one
-// B operand holds.
-constexpr int64_t kTilesEnough = 2048;
+// Up to 16 (down: 8) tokens, no expert has more columns than one B operand holds.
 template <int WT, int KS>
-tlhip_status gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
+void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
     const unsigned grid = slots * ((a.I / 16 + kWaves / KS - 1) / (kWaves / KS));
     const Layout at = layout<WT, 2, KS>(a.K / 32, a.M < 32 ? a.M : 32);
-    if (a.M <= 16) moe_gate_up_kernel<WT, KS, 1><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
-    else moe_gate_up_kernel<WT, KS, 2><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
-    return TLHIP_OK;
+    if (a.M == 1) moe_gate_up_kernel<WT, KS, 1, true><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    else if (a.M <= 16) moe_gate_up_kernel<WT, KS, 1, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    else moe_gate_up_kernel<WT, KS, 2, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
 }
 template <int WT, int KS>
-tlhip_status down(hipStream_t s, const MoeArgs& a, unsigned slots) {
+void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
     const unsigned grid = slots * ((a.K / 16 + kWaves / KS - 1) / (kWaves / KS));
     const Layout at = layout<WT, 1, KS>(a.I / 32, a.M < 16 ? 2 * a.M : 32);
     if (a.M <= 8) moe_down_kernel<WT, KS, 1><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     else moe_down_kernel<WT, KS, 2><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
-    return TLHIP_OK;
+}
+// Waves that share out the k of a tile of 16 rows: as few as leave two
+// workgroups of four waves for every CU (the more tiles a workgroup has, the
+// fewer times the columns are staged), and no fewer than LDS has room for.
+template <int WT, int NR>
+int waves_of_tile(int64_t tiles, int nb) {
+    if (tiles >= 2048 && layout<WT, NR, 1>(nb, 32).bytes <= kLdsDynamic) return 1;
+    if (tiles >= 1024 && layout<WT, NR, 2>(nb, 32).bytes <= kLdsDynamic) return 2;
+    return 4;
 }
 template <int WT>
-tlhip_status gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    if ((int64_t)slots * (a.I / 16) >= kTilesEnough && layout<WT, 2, 1>(a.K / 32, 32).bytes <= kLdsDynamic) return gate_up<WT, 1>(s, a, slots);
-    return gate_up<WT, 4>(s, a, slots);
+void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    switch (waves_of_tile<WT, 2>((int64_t)slots * (a.I / 16), a.K / 32)) {
+        case 1: return gate_up<WT, 1>(s, a, slots);
+        case 2: return gate_up<WT, 2>(s, a, slots);
+        default: return gate_up<WT, 4>(s, a, slots);
+    }
 }
 template <int WT>
-tlhip_status down(hipStream_t s, const MoeArgs& a, unsigned slots) {
+void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
     if (a.M == 1) {
         const Layout at = layout_one<WT>(a.I / 32, a.top);
         if (at.bytes <= kLdsDynamic) {
             moe_down_one_kernel<WT><<<a.K / 16, kOneWaves * 64, at.bytes, s>>>(a, at);
-            return TLHIP_OK;
+            return;
         }
     }
-    if ((int64_t)slots * (a.K / 16) >= kTilesEnough && layout<WT, 1, 1>(a.I / 32, 32).bytes <= kLdsDynamic) return down<WT, 1>(s, a, slots);
-    return down<WT, 4>(s, a, slots);
+    switch (waves_of_tile<WT, 1>((int64_t)slots * (a.K / 16), a.I / 32)) {
+        case 1: return down<WT, 1>(s, a, slots);
+        case 2: return down<WT, 2>(s, a, slots);
+        default: return down<WT, 4>(s, a, slots);
+    }
 }
 
 }  // namespace
@@ -725,12 +802,13 @@ tlhip_status down(hipStream_t s, const MoeArgs& a, unsigned slots) {
 tlhip_status launch_moe(hipStream_t s, const MoeArgs& a) {
     moe_router_kernel<<<a.M, 1024, 0, s>>>(a);
     const unsigned slots = a.M * a.top < a.E ? a.M * a.top : a.E;
-    if (a.wt_gu == TLHIP_F16) TLHIP_TRY(gate_up<TLHIP_F16>(s, a, slots));
-    else if (a.wt_gu == TLHIP_Q4_0) TLHIP_TRY(gate_up<TLHIP_Q4_0>(s, a, slots));
-    else TLHIP_TRY(gate_up<TLHIP_Q8_0>(s, a, slots));
-    if (a.wt_down == TLHIP_F16) return down<TLHIP_F16>(s, a, slots);
-    if (a.wt_down == TLHIP_Q4_0) return down<TLHIP_Q4_0>(s, a, slots);
-    return down<TLHIP_Q8_0>(s, a, slots);
+    if (a.wt_gu == TLHIP_F16) gate_up<TLHIP_F16>(s, a, slots);
+    else if (a.wt_gu == TLHIP_Q4_0) gate_up<TLHIP_Q4_0>(s, a, slots);
+    else gate_up<TLHIP_Q8_0>(s, a, slots);
+    if (a.wt_down == TLHIP_F16) down<TLHIP_F16>(s, a, slots);
+    else if (a.wt_down == TLHIP_Q4_0) down<TLHIP_Q4_0>(s, a, slots);
+    else down<TLHIP_Q8_0>(s, a, slots);
+    return TLHIP_OK;
 }
 
 }  // namespace tlhip
