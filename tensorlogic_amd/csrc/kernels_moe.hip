@@ -38,11 +38,12 @@ namespace {
 
 constexpr int kWaves = 4;                  // of a workgroup of the products
 constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
-// By the matrices of a product (gate and up: 2, down: 1): slots of weights that
-// a wave has in flight, and the columns staged in LDS at a time (or one round of
-// slots, if that is more).  Both leave room for two workgroups on a CU.
-constexpr int ring_slots(int nr) { return nr == 2 ? 2 : 4; }
-constexpr int column_budget(int nr) { return (nr == 2 ? 24 : 40) << 10; }
+// Slots of weights that a wave has in flight, and the columns staged in LDS at a
+// time (or one round of slots, if that is more): two workgroups fit on a CU with
+// rows of 5632.  (Deeper rings and more columns measured the same; with one
+// workgroup to a CU 13 tokens' down took 45 us instead of 33.)
+constexpr int kRing = 2;
+constexpr int kColumnBytes = 24 << 10;
 
 // ---------------------------------------------------------------------------
 // router
@@ -303,72 +304,76 @@ __device__ __forceinline__ int slot_expert(const MoeArgs& a, int slot, MoeShared
 
 // The columns of a product.  Column c of piece s of block b is 16 bytes at
 // (4 b + s) * ncol + c; past the row's nb blocks they are zeros.  A thread
-// loads four pieces before it stores any.
+// asks for the first kPieces of a chunk's pieces (fetch) while the chunk
+// before is multiplied, and stores them and the rest (put) after it.
+constexpr int kPieces = 4;
 __device__ __forceinline__ f4 low_part(const f4& p) {
     f4 r;
 #pragma unroll
     for (int k = 0; k < 4; k++) r[k] = p[k] - (float)(h16)p[k];
     return r;
 }
+template <typename LOADER>
+struct Stage : LOADER {
+    struct Ahead {
+        typename LOADER::Run p[kPieces], q[kPieces];
+    };
+    // pieces i0 + k * (threads of the workgroup)
+    __device__ __forceinline__ void load(Ahead& v, int i0, int c0, int blocks, int nb) const {
+        const uint32_t by_nt = 0xFFFFFFFFu / this->nt + 1;   // i / nt = umulhi(i, by_nt): i nt < 2^32
+#pragma unroll
+        for (int k = 0; k < kPieces; k++) {
+            const int i = i0 + k * kWaves * 64, bs = this->nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * this->nt, b = c0 + (bs >> 2);
+            v.p[k] = v.q[k] = typename LOADER::Run{};
+            if (i < blocks * 4 * this->nt && b < nb) this->get(v.p[k], v.q[k], t, b, bs & 3);
+        }
+    }
+    __device__ __forceinline__ void store(const Ahead& v, int i0, h8* cols, int blocks) const {
+#pragma unroll
+        for (int k = 0; k < kPieces; k++)
+            if (i0 + k * kWaves * 64 < blocks * 4 * this->nt) this->set(v.p[k], v.q[k], cols, i0 + k * kWaves * 64);
+    }
+    __device__ __forceinline__ void fetch(Ahead& v, int c0, int blocks, int nb) const { load(v, threadIdx.x, c0, blocks, nb); }
+    __device__ __forceinline__ void put(Ahead& v, h8* cols, int c0, int blocks, int nb) const {
+        store(v, threadIdx.x, cols, blocks);
+        for (int i0 = threadIdx.x + kPieces * kWaves * 64; i0 < blocks * 4 * this->nt; i0 += kPieces * kWaves * 64) {
+            load(v, i0, c0, blocks, nb);
+            store(v, i0, cols, blocks);
+        }
+    }
+};
 // Gate and up: x of the tokens list[0 .. nt), or of the only token.
 template <int WT, bool ONE>
-struct StageX {
+struct LoadX {
+    typedef h4 Run;
     const MoeArgs& a;
     const int* list;
     int nt;
     __device__ __forceinline__ int ncol() const { return nt; }
-    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
-        const uint32_t by_nt = 0xFFFFFFFFu / nt + 1;   // i / nt = umulhi(i, by_nt): i nt < 2^32
-        for (int i0 = threadIdx.x; i0 < blocks * 4 * nt; i0 += 4 * kWaves * 64) {
-            h4 p[4], q[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * kWaves * 64, bs = nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * nt, b = c0 + (bs >> 2);
-                p[k] = q[k] = h4{};
-                if (i < blocks * 4 * nt && b < nb) {
-                    const uint16_t* x = a.x + (ONE ? 0 : (size_t)(list[t] / a.top) * a.K) + b * 32;
-                    p[k] = *(const h4*)(x + run0<WT>(bs & 3));
-                    q[k] = *(const h4*)(x + run1<WT>(bs & 3));
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * kWaves * 64;
-                if (i < blocks * 4 * nt) cols[i] = piece<WT>(p[k], q[k]);
-            }
-        }
+    __device__ __forceinline__ void get(h4& p, h4& q, int t, int b, int s) const {
+        const uint16_t* x = a.x + (ONE ? 0 : (size_t)(list[t] / a.top) * a.K) + b * 32;
+        p = *(const h4*)(x + run0<WT>(s));
+        q = *(const h4*)(x + run1<WT>(s));
     }
+    __device__ __forceinline__ void set(const h4& p, const h4& q, h8* cols, int i) const { cols[i] = piece<WT>(p, q); }
 };
 // Down: hi and lo of each token's h 2^-e, one after the other.
 template <int WT>
-struct StageH {
+struct LoadH {
+    typedef f4 Run;
     const MoeArgs& a;
     const int* list;
     int nt;
     const float* scale;
     __device__ __forceinline__ int ncol() const { return 2 * nt; }
-    __device__ __forceinline__ void operator()(h8* cols, int c0, int blocks, int nb) const {
-        const uint32_t by_nt = 0xFFFFFFFFu / nt + 1;
-        for (int i0 = threadIdx.x; i0 < blocks * 4 * nt; i0 += 4 * kWaves * 64) {
-            f4 p[4], q[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * kWaves * 64, bs = nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * nt, b = c0 + (bs >> 2);
-                p[k] = q[k] = f4{0, 0, 0, 0};
-                if (i < blocks * 4 * nt && b < nb) {
-                    const float* h = a.h + (size_t)list[t] * a.I + b * 32;
-                    p[k] = *(const f4*)(h + run0<WT>(bs & 3)) * scale[t];
-                    q[k] = *(const f4*)(h + run1<WT>(bs & 3)) * scale[t];
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * kWaves * 64;
-                if (i >= blocks * 4 * nt) continue;
-                cols[2 * i] = piece<WT>(p[k], q[k]);
-                cols[2 * i + 1] = piece<WT>(low_part(p[k]), low_part(q[k]));
-            }
-        }
+    __device__ __forceinline__ void get(f4& p, f4& q, int t, int b, int s) const {
+        const float* h = a.h + (size_t)list[t] * a.I + b * 32;
+        p = *(const f4*)(h + run0<WT>(s)) * scale[t];
+        q = *(const f4*)(h + run1<WT>(s)) * scale[t];
+    }
+    __device__ __forceinline__ void set(const f4& p, const f4& q, h8* cols, int i) const {
+        cols[2 * i] = piece<WT>(p, q);
+        cols[2 * i + 1] = piece<WT>(low_part(p), low_part(q));
     }
 };
 
@@ -383,9 +388,9 @@ __host__ __device__ inline Layout layout(int nb, int max_cols) {
     constexpr int round = Slot<WT>::BLOCKS * KS;
     Layout l;
     const int whole = (nb + round - 1) / round * round * 64 * max_cols, least = round * 64 * max_cols;
-    l.column_bytes = whole < column_budget(NR) ? whole : column_budget(NR) > least ? column_budget(NR) : least;
+    l.column_bytes = whole < kColumnBytes ? whole : kColumnBytes > least ? kColumnBytes : least;
     l.ring_at = l.column_bytes;
-    l.scales_at = l.ring_at + kWaves * NR * ring_slots(NR) * Slot<WT>::BYTES;
+    l.scales_at = l.ring_at + kWaves * NR * kRing * Slot<WT>::BYTES;
     l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : kWaves / KS * NR * scale_bytes(nb));
     if (KS > 1 && l.bytes < kRedBytes) l.bytes = kRedBytes;
     return l;
@@ -400,7 +405,7 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
     using S = Slot<WT>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS;
     const int c16 = lane & 15, g = lane >> 4, ncol = stage.ncol();
-    constexpr int ROUND = S::BLOCKS * KS, kRing = ring_slots(NR);
+    constexpr int ROUND = S::BLOCKS * KS;
     int chunk = at.column_bytes / (64 * ncol) / ROUND * ROUND;   // blocks of a chunk: whole rounds of the KS waves' slots
     const int all = (nb + ROUND - 1) / ROUND * ROUND;
     if (chunk > all) chunk = all;
@@ -420,9 +425,11 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
 #pragma unroll
         for (int r = 0; r < NR; r++) w[r].copy(n, ring_lds + (k * NR + r) * S::BYTES);
     };
-    // One token's columns do not wait for the router's choice, which the copies
-    // do: they go first, and copies return in order.  Else the copies go first.
-    if constexpr (ONE) stage(cols, 0, chunk, nb);
+    // Loads return in order: the columns are asked for before the copies.  One
+    // token's do not even wait for the router's choice, which the copies do.
+    typename STAGE::Ahead ahead;
+    stage.fetch(ahead, 0, chunk, nb);
+    if constexpr (ONE) stage.put(ahead, cols, 0, chunk, nb);
     if constexpr (WT != TLHIP_F16) {
         const uint32_t scales_lds = __builtin_amdgcn_readfirstlane(lds_address(scales));
 #pragma unroll
@@ -432,18 +439,20 @@ __device__ __forceinline__ void multiply(const Rows<WT> (&w)[NR], const uint16_t
 #pragma unroll
     for (int k = 0; k < kRing; k++, next += KS)
         if (next < slots) copy(next, k);
-    if constexpr (ONE) {   // the scales have landed
+    auto scales_landed = [&]() {   // (their copies are older than the slots')
         if (next <= slots - 1 + KS) sk_wait_vm<kRing * NR * S::COPIES>();
         else sk_wait_vm<0>();
-    }
+    };
+    if constexpr (ONE) scales_landed();
     for (int c0 = 0; c0 < all; c0 += chunk) {
         const int blocks = all - c0 < chunk ? all - c0 : chunk;
-        if (!ONE || c0) {   // (its loads are waited for, so the scales have landed)
+        if (!ONE || c0) {
             lds_barrier();
-            stage(cols, c0, blocks, nb);
-            sk_wait_vm<0>();
+            stage.put(ahead, cols, c0, blocks, nb);
+            if (c0 == 0) scales_landed();
         }
         lds_barrier();
+        if (c0 + chunk < all) stage.fetch(ahead, c0 + chunk, min(all - c0 - chunk, chunk), nb);
         const int end = min((c0 + blocks) / S::BLOCKS, slots);
         for (int n = c0 / S::BLOCKS + part; n < end; n += KS) {
             // the slot has landed when no more copies are in flight than the
@@ -505,7 +514,7 @@ template <int WT, int CT, int KS, bool ONE>
 __device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds,
                                              MoeShared& sh, int one_pair = 0) {
     f4 acc[2][CT];
-    const StageX<WT, ONE> stage{a, sh.list + t0, nt};
+    const Stage<LoadX<WT, ONE>> stage{{a, sh.list + t0, nt}};
     const int tiles = a.I / 16, nb = a.K / 32;
     // (a wave past the last tile computes that one and stores nothing)
     const size_t row = (size_t)e * a.I + 16 * (tile < tiles ? tile : tiles - 1);
@@ -567,7 +576,7 @@ __device__ __forceinline__ float scale_for(float m) {
 template <int WT, int CT, int KS>
 __device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds, MoeShared& sh) {
     f4 acc[1][CT];
-    const StageH<WT> stage{a, sh.list + t0, nt, sh.scale + t0};
+    const Stage<LoadH<WT>> stage{{a, sh.list + t0, nt, sh.scale + t0}};
     const int tiles = a.K / 16, nb = a.I / 32;
     const size_t row = (size_t)e * a.K + 16 * (tile < tiles ? tile : tiles - 1);
     const Rows<WT> w[1] = {Rows<WT>(a.down, row, nb)};
@@ -745,7 +754,7 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
 constexpr int kLdsDynamic = 156 << 10;
 static_assert(kLdsDynamic + sizeof(MoeShared) <= 160 << 10, "LDS of a CU");
 static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "rows of a Q type fit");
-static_assert((40 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
+static_assert((32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
 
 // Up to 16 (down: 8) tokens, no expert has more columns than one B operand holds.
 template <int WT, int KS>
