@@ -23,6 +23,7 @@
 // of its scale, which is otherwise 0) and zeros, so a position that a query
 // does not see adds exactly nothing to it, and one that it sees shows.
 #include <cmath>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "internal.hpp"
@@ -222,10 +223,6 @@ __device__ __forceinline__ float rows4_max(float v) {   // over the lanes l, l ^
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
-__device__ __forceinline__ float rows4_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
 
 // Four bytes q + 128 -> f16 q: the byte under 0x64 is 1024 + q + 128.
 __device__ __forceinline__ void bytes_h4(uint32_t w, h2& a, h2& b) {
@@ -245,10 +242,10 @@ struct Kv8Wave {
     static constexpr int NC = (D + 31) / 32;   // 32-dim chunks, the last one maybe half
     h8 q[NQ][NC];
     f32x4 o[NQ][2 * NC];
-    float M[NQ], l[NQ];   // l: this lane's keys only, until the end
+    float M[NQ], l[NQ];   // the same in a row's four lanes
     int pos[NQ];
     int c16, g;
-    float sl;             // scale * log2(e)
+    float sl;             // |scale| * log2(e) (the queries carry its sign)
 
     static __device__ __forceinline__ bool chunk_ok(int c, int g) { return D % 32 == 0 || c < NC - 1 || g < 2; }
     static __device__ __forceinline__ bool dim_ok(int p, int c16) { return D % 32 == 0 || p < NC - 1 || c16 < 8; }
@@ -257,7 +254,8 @@ struct Kv8Wave {
         const int lane = threadIdx.x & 63;
         c16 = lane & 15;
         g = lane >> 4;
-        sl = p.scale * kLog2e;
+        sl = fabsf(p.scale) * kLog2e;
+        const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
             const int r = row0 + 16 * n + c16, rr = r < rows ? r : rows - 1;
@@ -266,8 +264,9 @@ struct Kv8Wave {
             const uint16_t* src = p.q + ((size_t)s * p.H + (size_t)head * p.group + hg) * D;
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                q[n][c] = h8{};
-                if (chunk_ok(c, g)) q[n][c] = *(const h8*)(src + 32 * c + 8 * g);
+                u4 v = {0, 0, 0, 0};
+                if (chunk_ok(c, g)) v = *(const u4*)(src + 32 * c + 8 * g) ^ sign;
+                q[n][c] = __builtin_bit_cast(h8, v);
             }
 #pragma unroll
             for (int t = 0; t < 2 * NC; t++) o[n][t] = f32x4{0, 0, 0, 0};
@@ -276,12 +275,14 @@ struct Kv8Wave {
         }
     }
 
-    // One tile: kx[c][t] the lane's keys (8 dims of chunk c of key 2 c16 + t),
-    // vx[t] its V^T rows; ks, lvs[8]: the factor of the score and what is
-    // added to it for the lane's keys 8g + 2i + t (index 4t + i), iv: 1 / vs.
-    template <typename KX, typename VX, typename LV>
-    __device__ __forceinline__ void tile(const KX& kx, const VX& vx, float ks, const LV& lvs, float iv, int key0,
-                                         bool masked) {
+    // One tile: kx(c, t) the lane's keys (8 dims of chunk c of key 2 c16 + t),
+    // vx(t) its V^T rows; f: the factor of the score; lv(i): log2 of V's scale
+    // at the lane's key i (8g + 2 (i & 3) + (i >> 2)); iv: 1 / that scale.
+    // Per score a maximum (two to an instruction), one fused operation, one
+    // exp and half a conversion; the weights' sum comes from the matrix cores
+    // (a row of ones), so that it is the sum of the weights as rounded.
+    template <bool MASK, bool EACH, typename KX, typename VX, typename LV>
+    __device__ __forceinline__ void tile(const KX& kx, const VX& vx, float f, const LV& lv, float iv, int key0) {
         f32x4 sc[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = f32x4{0, 0, 0, 0};
@@ -294,33 +295,45 @@ struct Kv8Wave {
                 for (int n = 0; n < NQ; n++)
                     sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[n][c], sc[n][t], 0, 0, 0);
             }
-        h8 pr[NQ];
-        const float f = sl * ks;
+        auto seen = [&](int n, int i) { return !MASK || key0 + 8 * g + 2 * (i & 3) + (i >> 2) <= pos[n]; };
+        float top[NQ];   // the lane's largest exponent
+        bool higher = false;
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-            float x[8], m = kNone;
+            float m = kNone;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[i] = fmaf(sc[n][i >> 2][i & 3], f, lvs(i));
-                if (masked && key0 + 8 * g + 2 * (i & 3) + (i >> 2) > pos[n]) x[i] = -INFINITY;
-                m = fmaxf(m, x[i]);
+                const float x = EACH ? fmaf(sc[n][i >> 2][i & 3], f, lv(i)) : sc[n][i >> 2][i & 3];
+                m = fmaxf(m, seen(n, i) ? x : kNone);
             }
-            m = rows4_max(m);
-            if (__any(m > M[n] + 8.0f)) {
-                const float mn = fmaxf(M[n], m), r = __builtin_amdgcn_exp2f(M[n] - mn);
+            top[n] = EACH ? m : fmaf(m, f, lv(0));
+            higher |= top[n] > M[n] + 8.0f;
+        }
+        if (__any(higher)) {
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                const float m = rows4_max(top[n]), mn = m > M[n] + 8.0f ? m : M[n], r = __builtin_amdgcn_exp2f(M[n] - mn);
                 M[n] = mn;
                 l[n] *= r;
 #pragma unroll
                 for (int t = 0; t < 2 * NC; t++) o[n][t] *= r;
             }
-            float sum = 0.0f;
+        }
+        h8 pr[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const float c = EACH ? -M[n] : lv(0) - M[n];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float w = __builtin_amdgcn_exp2f(x[i] - M[n]);
-                sum += w;
-                pr[n][i] = (h16)w;
+                const float x = fmaf(sc[n][i >> 2][i & 3], f, EACH ? lv(i) + c : c);
+                pr[n][i] = (h16)__builtin_amdgcn_exp2f(seen(n, i) ? x : -INFINITY);
             }
-            l[n] = fmaf(sum, iv, l[n]);
+        }
+        const h8 ones = {(h16)1.0f, (h16)1.0f, (h16)1.0f, (h16)1.0f, (h16)1.0f, (h16)1.0f, (h16)1.0f, (h16)1.0f};
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pr[n], f32x4{0, 0, 0, 0}, 0, 0, 0);
+            l[n] = fmaf(s[0], iv, l[n]);
         }
 #pragma unroll
         for (int t = 0; t < 2 * NC; t++) {
@@ -330,18 +343,22 @@ struct Kv8Wave {
         }
     }
 
-    // Tiles t0, t0 + step, ... below t1 (tile nfull, if among them, is the tail).
-    __device__ __forceinline__ void walk(const Kv8Attn& p, int head, int t0, int t1, int step, int row_first_pos) {
-        const uint8_t* kq = p.kq + (size_t)head * p.n_blocks * 32 * D;
-        const uint8_t* vq = p.vq + (size_t)head * p.n_blocks * 32 * D;
+    // Tiles t0, t0 + step, ... below t1 (tile nfull, if among them, is the
+    // tail).  pos0: the first row's position, which sees whole tiles below it.
+    __device__ __forceinline__ void walk(const Kv8Attn& p, int head, int t0, int t1, int step, int pos0) {
+        const uint8_t* kq = p.kq + (size_t)head * p.n_blocks * 32 * D + (g * 32 + 2 * c16) * 8;
+        const uint8_t* vq = p.vq + (size_t)head * p.n_blocks * 32 * D + (c16 * 4 + g) * 16;
         const float* ks = p.ks + (size_t)head * p.n_blocks;
         const float* vs = p.vs + (size_t)head * p.n_blocks;
         const int tq = t1 < p.n_full ? t1 : p.n_full;
         int t = t0;
         u4 kr[NC], vr[NC];
+        float fk = 0.0f, fv = 1.0f;
         auto load = [&](int b) {
-            const uint8_t* kb = kq + (size_t)b * 32 * D + (g * 32 + 2 * c16) * 8;
-            const uint8_t* vb = vq + (size_t)b * 32 * D + (c16 * 4 + g) * 16;
+            const uint8_t* kb = kq + (size_t)b * 32 * D;
+            const uint8_t* vb = vq + (size_t)b * 32 * D;
+            fk = ks[b];
+            fv = vs[b];
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 kr[c] = u4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
@@ -350,21 +367,23 @@ struct Kv8Wave {
                 if (dim_ok(c, c16)) vr[c] = *(const u4*)(vb + c * 16 * 4 * 16);
             }
         };
-        if (t < tq) load(t);
-        for (; t < tq; t += step) {
+        auto step_over = [&](auto mask, int b, int next) {
             u4 kc[NC], vc[NC];
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 kc[c] = kr[c];
                 vc[c] = vr[c];
             }
-            const float fk = ks[t], fv = vs[t];
-            if (t + step < tq) load(t + step);
-            const float lv = __builtin_amdgcn_logf(fv);
-            tile([&](int c, int h) { return bytes_h8(kc[c][2 * h], kc[c][2 * h + 1]); },
-                 [&](int h) { return bytes_h8(vc[h >> 1][2 * (h & 1)], vc[h >> 1][2 * (h & 1) + 1]); }, fk,
-                 [&](int) { return lv; }, 1.0f / fv, 32 * t, 32 * t + 31 > row_first_pos);
-        }
+            const float f = sl * fk, lv = __builtin_amdgcn_logf(fv), iv = __builtin_amdgcn_rcpf(fv);
+            if (next < tq) load(next);
+            tile<decltype(mask)::value, false>([&](int c, int h) { return bytes_h8(kc[c][2 * h], kc[c][2 * h + 1]); },
+                                               [&](int h) { return bytes_h8(vc[h >> 1][2 * (h & 1)], vc[h >> 1][2 * (h & 1) + 1]); }, f,
+                                               [&](int) { return lv; }, iv, 32 * b);
+        };
+        if (t < tq) load(t);
+        const int whole = (pos0 + 1) >> 5;   // tiles below it are seen by every row
+        for (; t < tq && t < whole; t += step) step_over(std::false_type{}, t, t + step);
+        for (; t < tq; t += step) step_over(std::true_type{}, t, t + step);
         if (t < t1) {   // the tail: f16 values
             const size_t th = (size_t)p.tail_cur * p.n_kv + head;
             const uint16_t* kt = p.tail_k + th * 32 * D;
@@ -373,17 +392,18 @@ struct Kv8Wave {
             float lv[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) lv[i] = fl[2 * (i & 3) + (i >> 2)];
-            tile([&](int c, int h) {
-                     h8 a = {};
-                     if (chunk_ok(c, g)) a = *(const h8*)(kt + ((4 * c + g) * 32 + 2 * c16 + h) * 8);
-                     return a;
-                 },
-                 [&](int h) {
-                     h8 a = {};
-                     if (dim_ok(h >> 1, c16)) a = *(const h8*)(vt + ((((h >> 1) * 16 + c16) * 4 + g) * 2 + (h & 1)) * 8);
-                     return a;
-                 },
-                 1.0f, [&](int i) { return lv[i]; }, 1.0f, 32 * t, true);
+            tile<true, true>(
+                [&](int c, int h) {
+                    h8 a = {};
+                    if (chunk_ok(c, g)) a = *(const h8*)(kt + ((4 * c + g) * 32 + 2 * c16 + h) * 8);
+                    return a;
+                },
+                [&](int h) {
+                    h8 a = {};
+                    if (dim_ok(h >> 1, c16)) a = *(const h8*)(vt + ((((h >> 1) * 16 + c16) * 4 + g) * 2 + (h & 1)) * 8);
+                    return a;
+                },
+                sl, [&](int i) { return lv[i]; }, 1.0f, 32 * t);
         }
     }
 
@@ -392,7 +412,7 @@ struct Kv8Wave {
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
             const int r = row0 + 16 * n + c16;
-            const float inv = 1.0f / rows4_sum(l[n]);
+            const float inv = 1.0f / l[n];
             if (r >= rows) continue;
             const int s = r / p.group, hg = r - s * p.group;
             uint16_t* dst = p.out + ((size_t)s * p.H + (size_t)head * p.group + hg) * D;
@@ -411,14 +431,21 @@ struct Kv8Wave {
     }
 };
 
-// Many rows: a wave per NQ * 16 rows, four to a workgroup, each over all its keys.
+// Many rows: a wave per NQ * 16 rows, four to a workgroup, each over all its
+// keys.  Later rows see more keys: the workgroups of a round (those that start
+// together, one to a CU) go down from the longest, those of the next round up,
+// so that a CU's share is about the same everywhere.
 template <int D, int NQ>
-__global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Kv8Attn p) {
-    const int rows = p.S * p.group;
-    const int head = blockIdx.x % p.n_kv;
-    // the rows with the most keys first
-    const int tile = (int)(gridDim.x / p.n_kv) - 1 - blockIdx.x / p.n_kv;
-    const int row0 = (tile * 4 + (threadIdx.x >> 6)) * (16 * NQ);
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_rows_kernel(Kv8Attn p) {
+    constexpr int ROUND = 256;
+    const int rows = p.S * p.group, wgs = gridDim.x;
+    int at = blockIdx.x;   // the place in falling order
+    if (at / ROUND & 1) {
+        const int first = at / ROUND * ROUND, last = (first + ROUND < wgs ? first + ROUND : wgs) - 1;
+        at = first + last - at;
+    }
+    const int head = at % p.n_kv, tile = wgs / p.n_kv - 1 - at / p.n_kv;
+    const int row0 = (tile * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (16 * NQ);
     if (row0 >= rows) return;
     const int row1 = row0 + 16 * NQ < rows ? row0 + 16 * NQ : rows;
     Kv8Wave<D, NQ> w;
@@ -431,7 +458,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Kv8Attn p) {
 // workgroup's four waves, which join through LDS; the splits' sums go to
 // scratch for kv8_join_kernel.
 template <int D, int NQ>
-__global__ __launch_bounds__(256) void kv8_attn_keys_kernel(Kv8Attn p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_keys_kernel(Kv8Attn p) {
     constexpr int NC = (D + 31) / 32;
     __shared__ float so[4][16 * NQ][NC * 32 + 4];
     __shared__ float sm[4][16 * NQ], sl[4][16 * NQ];
@@ -439,19 +466,19 @@ __global__ __launch_bounds__(256) void kv8_attn_keys_kernel(Kv8Attn p) {
     const int split = blockIdx.x % p.splits, head = blockIdx.x / p.splits % p.n_kv;
     const int row0 = (int)(blockIdx.x / p.splits / p.n_kv) * (16 * NQ);
     const int row1 = row0 + 16 * NQ < rows ? row0 + 16 * NQ : rows;
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Kv8Wave<D, NQ> w;
     w.init(p, head, row0, rows);
     const int tiles = ((p.q_pos0 + (row1 - 1) / p.group) >> 5) + 1;
     w.walk(p, head, split * 4 + wave, tiles, 4 * p.splits, p.q_pos0 + row0 / p.group);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
-        const float l = rows4_sum(w.l[n]);
         const int r = 16 * n + w.c16;
         if (w.g == 0) {
             sm[wave][r] = w.M[n];
-            sl[wave][r] = l;
+            sl[wave][r] = w.l[n];
         }
+        if (row0 + r >= rows) continue;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -494,26 +521,55 @@ __global__ __launch_bounds__(256) void kv8_attn_keys_kernel(Kv8Attn p) {
     }
 }
 
-// The splits of one row joined: a wave per (head, row), a lane per D / 64 dims.
+// The splits of one (head, row) joined by a workgroup: a thread loads 4 dims of
+// one split at a time, all splits' loads in flight together, and the threads
+// of the same dims add up in a fixed order through LDS.
 template <int D>
-__global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn p) {
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attn p) {
+    constexpr int Q = D / 4, PER = 256 / Q;   // threads of a split, splits at a time
+    __shared__ f32x4 so[256];
+    __shared__ float sl[PER];
     const int rows = p.S * p.group;
     const int row = blockIdx.x % rows, head = blockIdx.x / rows;
     const float* src = p.scratch + ((size_t)head * rows + row) * p.splits * (D + 4);
     float M = kNone;
-    for (int k = 0; k < p.splits; k++) M = fmaxf(M, src[(size_t)k * (D + 4) + D]);
-    const int s = row / p.group, hg = row - s * p.group;
-    uint16_t* dst = p.out + ((size_t)s * p.H + (size_t)head * p.group + hg) * D;
-    for (int d = threadIdx.x; d < D; d += 64) {
-        float o = 0.0f, l = 0.0f;
-        for (int k = 0; k < p.splits; k++) {
-            const float* x = src + (size_t)k * (D + 4);
-            const float f = __builtin_amdgcn_exp2f(x[D] - M);
-            o = fmaf(x[d], f, o);
-            l = fmaf(x[D + 1], f, l);
+    for (int k = threadIdx.x & 63; k < p.splits; k += 64) M = fmaxf(M, src[(size_t)k * (D + 4) + D]);
+    const int part = threadIdx.x / Q, d = threadIdx.x % Q;
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0.0f;
+    constexpr int AHEAD = 4;
+    for (int k0 = 0; k0 < p.splits; k0 += AHEAD * PER) {
+        f32x4 x[AHEAD], ml[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int k = k0 + a * PER + part;
+            const float* at = src + (size_t)(k < p.splits ? k : 0) * (D + 4);
+            x[a] = *(const f32x4*)(at + 4 * d);
+            ml[a] = *(const f32x4*)(at + D);
         }
-        dst[d] = f2h(o / l);
+        if (k0 == 0) M = wave_max(M);
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            if (part >= PER || k0 + a * PER + part >= p.splits) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[a][0] - M);
+            l = fmaf(ml[a][1], f, l);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = fmaf(x[a][j], f, o[j]);
+        }
     }
+    so[threadIdx.x] = o;
+    if (d == 0 && part < PER) sl[part] = l;
+    __syncthreads();
+    if (threadIdx.x >= Q) return;
+    for (int k = 1; k < PER; k++) {
+        o += so[k * Q + threadIdx.x];
+        l += sl[k];
+    }
+    const int s = row / p.group, hg = row - s * p.group;
+    uint16_t* dst = p.out + ((size_t)s * p.H + (size_t)head * p.group + hg) * D + 4 * threadIdx.x;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 4; j++) dst[j] = f2h(o[j] * inv);
 }
 
 template <int D>
@@ -521,16 +577,17 @@ tlhip_status attn_d(hipStream_t s, Kv8Attn p, const Kv8Plan& pl) {
     const int rows = p.S * p.group;
     if (pl.splits == 0) {
         const int wg = (rows + 64 * pl.nq - 1) / (64 * pl.nq) * p.n_kv;
+        if constexpr (D <= 128)
+            if (pl.nq == 2) kv8_attn_rows_kernel<D, 2><<<wg, 256, 0, s>>>(p);
         if (pl.nq == 1) kv8_attn_rows_kernel<D, 1><<<wg, 256, 0, s>>>(p);
-        else if (pl.nq == 2) kv8_attn_rows_kernel<D, 2><<<wg, 256, 0, s>>>(p);
-        else kv8_attn_rows_kernel<D, 4><<<wg, 256, 0, s>>>(p);
         return TLHIP_OK;
     }
     p.splits = pl.splits;
     const int wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * p.n_kv * pl.splits;
+    if constexpr (D <= 128)
+        if (pl.nq == 2) kv8_attn_keys_kernel<D, 2><<<wg, 256, 0, s>>>(p);
     if (pl.nq == 1) kv8_attn_keys_kernel<D, 1><<<wg, 256, 0, s>>>(p);
-    else kv8_attn_keys_kernel<D, 2><<<wg, 256, 0, s>>>(p);
-    if (pl.splits > 1) kv8_join_kernel<D><<<rows * p.n_kv, 64, 0, s>>>(p);
+    if (pl.splits > 1) kv8_join_kernel<D><<<rows * p.n_kv, 256, 0, s>>>(p);
     return TLHIP_OK;
 }
 
@@ -576,17 +633,12 @@ Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     Kv8Plan pl;
     const int64_t rows = (int64_t)S * group;
     const int tiles = (len + 31) / 32;
-    const int nq = rows <= 16 || D > 128 ? 1 : D > 64 ? 2 : 4;
-    const int64_t waves = (rows + 16 * nq - 1) / (16 * nq) * n_kv;
-    if (waves >= 1024) {
-        pl.nq = nq;
-        return pl;
-    }
     pl.nq = rows <= 16 || D > 128 ? 1 : 2;
     const int64_t wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * n_kv;
+    if (wg >= 1024) return pl;
     int64_t splits = 1024 / wg;
     if (splits < 1) splits = 1;
-    if (splits > (tiles + 7) / 8) splits = (tiles + 7) / 8;
+    if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
     pl.splits = (int)splits;
     pl.scratch_bytes = splits > 1 ? (size_t)n_kv * rows * splits * (D + 4) * sizeof(float) : 0;
     return pl;
