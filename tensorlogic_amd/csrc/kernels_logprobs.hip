@@ -145,23 +145,26 @@ struct TopShared {
     uint64_t group[64];
     uint64_t list[kList], ranked[kRanked];
     uint64_t best[4];
+    int above[4][64], rank[kRanked];
     int count, kept;
 };
 
 // The n-th largest of the 64 groups' keys (0 if there are fewer), the same in
-// every thread.
+// every thread: a lane stands for a group, and each wave counts the keys above
+// it among a quarter of them.
 __device__ __forceinline__ uint64_t bound(uint64_t mine, int n, TopShared& sh) {
     for (int k = 1; k < 4; k <<= 1) mine = max64(mine, __shfl_xor((unsigned long long)mine, k, 64));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
-    if ((threadIdx.x & 3) == 0) sh.group[threadIdx.x >> 2] = mine;
+    if ((lane & 3) == 0) sh.group[threadIdx.x >> 2] = mine;
     __syncthreads();
-    const uint64_t g = sh.group[threadIdx.x & 63];
+    const uint64_t g = sh.group[lane];
     int above = 0;
-#pragma unroll 8
-    for (int k = 0; k < 64; k++) {
-        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)g, k), hi = __builtin_amdgcn_readlane((int)(g >> 32), k);
-        above += ((uint64_t)hi << 32 | lo) > g;
-    }
+#pragma unroll
+    for (int k = 0; k < 16; k++) above += sh.group[16 * wave + k] > g;
+    sh.above[wave][lane] = above;
+    __syncthreads();
+    above = sh.above[0][lane] + sh.above[1][lane] + sh.above[2][lane] + sh.above[3][lane];
     const uint64_t who = __ballot(above == n - 1 && g != 0);
     if (!who) return 0;
     const int src = __builtin_ctzll(who);
@@ -169,15 +172,27 @@ __device__ __forceinline__ uint64_t bound(uint64_t mine, int n, TopShared& sh) {
     return (uint64_t)hi << 32 | lo;
 }
 
-// Writes the n largest of `count` keys in LDS to out in falling order, by
-// counting for each the keys above it.
-__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int n, uint64_t* out) {
-    for (int i = threadIdx.x; i < count; i += 256) {
-        const uint64_t k = keys[i];
+// Writes the n largest of `count` keys in LDS (0: none) to out in falling
+// order, by counting for each the keys above it: a wave per quarter of them.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int n, uint64_t* out, int* rank) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < count; i += 256) rank[i] = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < count; i0 += 64) {
+        const uint64_t k = i0 + lane < count ? keys[i0 + lane] : 0;
         int above = 0;
-        for (int j = 0; j < count; j++) above += keys[j] > k;
-        if (k && above < n) out[above] = k;
+        for (int j0 = 4 * wave; j0 < count; j0 += 16) {
+            uint64_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = j0 + j < count ? keys[j0 + j] : 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) above += o[j] > k;
+        }
+        if (i0 + lane < count && above) atomicAdd(&rank[i0 + lane], above);
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += 256)
+        if (keys[i] && rank[i] < n) out[rank[i]] = keys[i];
 }
 
 // The same by n rounds of the largest key below the last one; key(i), i <
@@ -247,22 +262,24 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         for (int j = 0; j < 32; j++) s.add(x[j]);
         if constexpr (TOP) {
             if (Batch<F32>::index(0) < have && (!best || m > key_value(best))) {
-                int first = 0;
+                int first = 31;   // (-inf past the row's end: behind every index of the row)
 #pragma unroll
-                for (int j = 31; j >= 0; j--) first = x[j] == m && Batch<F32>::index(j) < have ? Batch<F32>::index(j) : first;
-                best = key_of(m, begin + b + first);
+                for (int j = 30; j >= 0; j--) first = x[j] == m ? j : first;
+                best = key_of(m, begin + b + Batch<F32>::index(first));
             }
             if (nb == 0) tau = bound(best, a.n_top, sh);
-            if (m >= key_value(tau) || !tau) {
+            const float least = tau ? key_value(tau) : -INFINITY;
+            if (m >= least) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const int i = Batch<F32>::index(j);
-                    const uint64_t k = key_of(x[j], begin + b + i);
-                    if (i < have && k >= tau) {
-                        const int slot = atomicAdd(&sh.count, 1);
-                        if (slot < kList) sh.list[slot] = k;
+                for (int j = 0; j < 32; j++)
+                    if (x[j] >= least) {
+                        const int i = Batch<F32>::index(j);
+                        const uint64_t k = key_of(x[j], begin + b + i);
+                        if (i < have && k >= tau) {
+                            const int slot = atomicAdd(&sh.count, 1);
+                            if (slot < kList) sh.list[slot] = k;
+                        }
                     }
-                }
             }
             if (nb && !(nb & (nb + 1)) && b + kBatch < count) tau = bound(best, a.n_top, sh);
         }
@@ -273,7 +290,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     s = st[0];
     for (int k = 1; k < 4; k++) s.join(st[k]);
     if constexpr (TOP) {
-        tau = bound(best, a.n_top, sh);
+        if (count > kBatch) tau = bound(best, a.n_top, sh);   // (else it stands)
         const int listed = sh.count;
         if (listed <= kList) {
             for (int i = tid; i < listed; i += 256) {
@@ -285,7 +302,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
             }
             __syncthreads();
             const int kept = sh.kept;
-            if (kept <= kRanked) rank_keys(sh.ranked, kept, a.n_top, top);
+            if (kept <= kRanked) rank_keys(sh.ranked, kept, a.n_top, top, sh.rank);
             else rounds([&](int i) { return sh.list[i]; }, listed, a.n_top, top, sh);
         } else {
             rounds([&](int i) { return key_of(at<F32>(a, base + i), begin + i); }, count, a.n_top, top, sh);
@@ -304,6 +321,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 template <bool F32>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
     __shared__ uint64_t keys[kMaxChunks * kMaxTop], top[kMaxTop];
+    __shared__ int rank[kMaxChunks * kMaxTop];
     const int row = blockIdx.x, n = a.chunks * a.n_top;
     for (int i = threadIdx.x; i < n; i += 256) keys[i] = a.part_keys[(size_t)row * n + i];
     Stat<F32> s = Stat<F32>::none();
@@ -317,7 +335,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
         s.join(o);
     }
     __syncthreads();
-    rank_keys(keys, n, a.n_top, top);
+    rank_keys(keys, n, a.n_top, top, rank);
     __syncthreads();
     finish<F32>(a, row, s, top);
 }
@@ -326,10 +344,11 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
 
 // Chunks of a row: enough workgroups for two to a CU, and no more than one for
 // each batch of a row.
+constexpr int kWorkgroups = 512;
 LogprobPlan logprobs_plan(int rows, int V, int n_top) {
     LogprobPlan p;
     const int64_t batches = ((int64_t)V + kBatch - 1) / kBatch;
-    int64_t chunks = rows >= 512 ? 1 : (512 + rows - 1) / rows;
+    int64_t chunks = rows >= kWorkgroups ? 1 : (kWorkgroups + rows - 1) / rows;
     if (chunks > batches) chunks = batches;
     if (chunks > kMaxChunks) chunks = kMaxChunks;
     const int64_t per = (batches + chunks - 1) / chunks;
