@@ -112,31 +112,46 @@ struct Batch {
         if constexpr (F32) return f[j];
         else return (float)h[j / 8][j % 8];
     }
-    // elements base + index(j); -inf past `have` elements
-    __device__ __forceinline__ void load(const LogprobArgs& a, size_t base, int have) {
+    // Elements base + index(j), a batch of the row.  (No branch among the
+    // loads: each would wait for those before it.)
+    __device__ __forceinline__ void load(const LogprobArgs& a, size_t base) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const size_t i = base + (v * 256 + (int)threadIdx.x) * W;
+            if constexpr (F32) {
+                const f4_any w = *(const f4_any*)((const float*)a.x + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[4 * v + e] = w.f[e];
+            } else {
+                const h8_any w = *(const h8_any*)((const uint16_t*)a.x + i);
+                h[v] = __builtin_bit_cast(h8, u4{w.w[0], w.w[1], w.w[2], w.w[3]});
+            }
+        }
+    }
+    // The same of a row of `have` elements, less than a batch; -inf past them.
+    __device__ __forceinline__ void load_short(const LogprobArgs& a, size_t base, int have) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int i = (v * 256 + (int)threadIdx.x) * W;
-            if constexpr (F32) {
-                const float* p = (const float*)a.x + base + i;
-                if (i + W <= have) {
-                    const f4_any w = *(const f4_any*)p;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) f[4 * v + e] = w.f[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) f[4 * v + e] = i + e < have ? p[e] : -INFINITY;
-                }
-            } else {
-                const uint16_t* p = (const uint16_t*)a.x + base + i;
-                if (i + W <= have) {
-                    const h8_any w = *(const h8_any*)p;
-                    h[v] = __builtin_bit_cast(h8, u4{w.w[0], w.w[1], w.w[2], w.w[3]});
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) h[v][e] = i + e < have ? __builtin_bit_cast(h16, p[e]) : (h16)-INFINITY;
-                }
+            for (int e = 0; e < W; e++) {
+                if constexpr (F32) f[4 * v + e] = -INFINITY;
+                else h[v][e] = (h16)-INFINITY;
             }
+            if (i >= have) continue;
+#pragma unroll
+            for (int e = 0; e < W; e++) {
+                if constexpr (F32) f[4 * v + e] = i + e < have ? ((const float*)a.x)[base + i + e] : -INFINITY;
+                else h[v][e] = i + e < have ? __builtin_bit_cast(h16, ((const uint16_t*)a.x)[base + i + e]) : (h16)-INFINITY;
+            }
+        }
+    }
+    // -inf in place of the elements before index lo
+    __device__ __forceinline__ void drop_before(int lo) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            if constexpr (F32) f[j] = index(j) < lo ? -INFINITY : f[j];
+            else h[j / 8][j % 8] = index(j) < lo ? (h16)-INFINITY : h[j / 8][j % 8];
         }
     }
 };
@@ -251,9 +266,13 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         if (tid == 0) sh.count = sh.kept = 0;
     }
     for (int b = 0, nb = 0; b < count; b += kBatch, nb++) {
-        const int have = count - b;
+        // The last batch of several is moved back to be whole: its elements
+        // from lo on are new.  A row shorter than a batch ends at hi.
+        const int at0 = count - b < kBatch && nb ? count - kBatch : b, lo = b - at0, hi = count - at0;
         Batch<F32> x;
-        x.load(a, base + b, have);
+        if (hi >= kBatch) x.load(a, base + at0);
+        else x.load_short(a, base, hi);
+        if (lo) x.drop_before(lo);
         float m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 32; j++) m = fmaxf(m, x[j]);
@@ -261,11 +280,17 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int j = 0; j < 32; j++) s.add(x[j]);
         if constexpr (TOP) {
-            if (Batch<F32>::index(0) < have && (!best || m > key_value(best))) {
-                int first = 31;   // (-inf past the row's end: behind every index of the row)
+            auto mine = [&](int j) { return Batch<F32>::index(j) >= lo && Batch<F32>::index(j) < hi; };
+            if ((!best || m > key_value(best)) && (mine(0) || mine(31))) {
+                // the first element that is m (an -inf in place of another is none)
+                int first = -1;
+                if (m > -INFINITY) {
 #pragma unroll
-                for (int j = 30; j >= 0; j--) first = x[j] == m ? j : first;
-                best = key_of(m, begin + b + Batch<F32>::index(first));
+                    for (int j = 31; j >= 0; j--) first = x[j] == m ? j : first;
+                } else {
+                    for (int j = 31; j >= 0; j--) first = x[j] == m && mine(j) ? j : first;
+                }
+                if (first >= 0) best = key_of(m, begin + at0 + Batch<F32>::index(first));
             }
             if (nb == 0) tau = bound(best, a.n_top, sh);
             const float least = tau ? key_value(tau) : -INFINITY;
@@ -273,9 +298,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
                     if (x[j] >= least) {
-                        const int i = Batch<F32>::index(j);
-                        const uint64_t k = key_of(x[j], begin + b + i);
-                        if (i < have && k >= tau) {
+                        const uint64_t k = key_of(x[j], begin + at0 + Batch<F32>::index(j));
+                        if (mine(j) && k >= tau) {
                             const int slot = atomicAdd(&sh.count, 1);
                             if (slot < kList) sh.list[slot] = k;
                         }
