@@ -65,7 +65,10 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
     constexpr int PIECES = 4 * D;            // 8 values each
     constexpr int PT = (PIECES + 255) / 256; // pieces of a thread
     __shared__ float red[4];
-    __shared__ __align__(16) uint8_t tile[32 * D];
+    __shared__ __align__(16) uint8_t tile[34 * D];
+    // the tile in LDS, 16 bytes between every 256: neighbouring lanes' pieces
+    // lie 256 bytes apart in it and would share their banks
+    auto lds = [](int at) { return at + (at >> 8) * 16; };
     const int is_v = blockIdx.x & 1;
     const int head = (blockIdx.x >> 1) % p.n_kv, unit = (blockIdx.x >> 1) / p.n_kv;
     const int tid = threadIdx.x;
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
         for (int e = 0; e < 8; e++) q[e] = bad ? 128 : (uint8_t)((int)rintf((float)x[j][e] * inv) + 128);
         if (is_v) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) tile[v_at(key, 8 * u + e)] = q[e];
+            for (int e = 0; e < 8; e++) tile[lds(v_at(key, 8 * u + e))] = q[e];
         } else {
             uint32_t lo = 0, hi = 0;
 #pragma unroll
@@ -153,13 +156,13 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
                 lo |= (uint32_t)q[e] << (8 * e);
                 hi |= (uint32_t)q[4 + e] << (8 * e);
             }
-            *(u2v*)(tile + k_at(key, 8 * u)) = u2v{lo, hi};
+            *(u2v*)(tile + lds(k_at(key, 8 * u))) = u2v{lo, hi};
         }
     }
     __syncthreads();
     const size_t bt = (size_t)head * p.n_blocks + block;
     uint8_t* dst = (is_v ? p.vq : p.kq) + bt * 32 * D;
-    for (int i = tid; i < 2 * D; i += 256) *(u4*)(dst + 16 * i) = *(const u4*)(tile + 16 * i);
+    for (int i = tid; i < 2 * D; i += 256) *(u4*)(dst + 16 * i) = *(const u4*)(tile + lds(16 * i));
     if (tid == 0) (is_v ? p.vs : p.ks)[bt] = scale;
 }
 
