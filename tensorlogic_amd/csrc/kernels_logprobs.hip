@@ -158,7 +158,8 @@ struct Batch {
 
 struct TopShared {
     uint64_t group[64];
-    uint64_t list[kList], ranked[kRanked];
+    uint64_t ranked[kRanked];
+    int list[kList];   // elements of the row
     uint64_t best[4];
     int above[4][64], rank[kRanked];
     int count, kept;
@@ -295,15 +296,23 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
             if (nb == 0) tau = bound(best, a.n_top, sh);
             const float least = tau ? key_value(tau) : -INFINITY;
             if (m >= least) {
+                // the places of the batch's keys from tau up go to the list
+                uint32_t hit = 0, even = 0;
 #pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (x[j] >= least) {
-                        const uint64_t k = key_of(x[j], begin + at0 + Batch<F32>::index(j));
-                        if (mine(j) && k >= tau) {
-                            const int slot = atomicAdd(&sh.count, 1);
-                            if (slot < kList) sh.list[slot] = k;
-                        }
-                    }
+                for (int j = 0; j < 32; j++) {
+                    hit |= x[j] > least ? 1u << j : 0;
+                    even |= x[j] == least ? 1u << j : 0;
+                }
+                const int last = tau ? key_index(tau) - begin - at0 : kBatch;
+                for (; even; even &= even - 1) {
+                    const int j = __builtin_ctz(even), i = Batch<F32>::index(j);
+                    if (i >= lo && i < hi && i <= last) hit |= 1u << j;
+                }
+                if (hit) {
+                    int slot = atomicAdd(&sh.count, __builtin_popcount(hit));
+                    for (; hit; hit &= hit - 1, slot++)
+                        if (slot < kList) sh.list[slot] = at0 + Batch<F32>::index(__builtin_ctz(hit));
+                }
             }
             if (nb && !(nb & (nb + 1)) && b + kBatch < count) tau = bound(best, a.n_top, sh);
         }
@@ -316,9 +325,10 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     if constexpr (TOP) {
         if (count > kBatch) tau = bound(best, a.n_top, sh);   // (else it stands)
         const int listed = sh.count;
+        auto listed_key = [&](int i) { return key_of(at<F32>(a, base + sh.list[i]), begin + sh.list[i]); };
         if (listed <= kList) {
             for (int i = tid; i < listed; i += 256) {
-                const uint64_t k = sh.list[i];
+                const uint64_t k = listed_key(i);
                 if (k >= tau) {
                     const int slot = atomicAdd(&sh.kept, 1);
                     if (slot < kRanked) sh.ranked[slot] = k;
@@ -327,7 +337,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
             __syncthreads();
             const int kept = sh.kept;
             if (kept <= kRanked) rank_keys(sh.ranked, kept, a.n_top, top, sh.rank);
-            else rounds([&](int i) { return sh.list[i]; }, listed, a.n_top, top, sh);
+            else rounds(listed_key, listed, a.n_top, top, sh);
         } else {
             rounds([&](int i) { return key_of(at<F32>(a, base + i), begin + i); }, count, a.n_top, top, sh);
         }
