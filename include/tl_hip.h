@@ -284,7 +284,7 @@ tlhip_status tlhip_temperature_sample(tlhip_ctx ctx, tlhip_tensor logits, float 
  * entropy and top_logprob are F32.  -inf logits have probability 0 and their
  * log probability is -inf.  A row with a NaN or +inf, or of -inf alone, has
  * no distribution: NaN, and top_ids -1.  An id outside [0, V) gives NaN.
- * n_top <= min(64, V).                                                     */
+ * n_top <= min(64, V), V <= 2^30, fewer than 2^24 rows.                    */
 tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tensor ids, int n_top,
                                   tlhip_tensor logprob, tlhip_tensor entropy, tlhip_tensor top_logprob,
                                   tlhip_tensor top_ids);
@@ -297,10 +297,10 @@ tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tens
  * x and y [M, K], router [E, K], all f16; gate and up [E * I, K] and down
  * [E * K, I], the experts' rows one after another (f16 also [E, I, K] and
  * [E, K, I]), each F16, Q4_0 or Q8_0, gate and up of one type.  K and I are
- * multiples of 32 up to 16384, E <= 256, top_k <= min(E, 32).  The weights count as the
- * f16 values that linear() reads them as; what lies between x and y is not
- * rounded to f16.  y may be x.  Any M; the weights an expert's tokens need
- * are read once for up to 256 tokens.                                      */
+ * multiples of 32 up to 16384, E <= 256, top_k <= min(E, 32).  The weights
+ * count as the f16 values that linear() reads them as; what lies between x
+ * and y is not rounded to f16.  y may be x.  Any M; the weights an expert's
+ * tokens need are read once for up to 256 tokens.                          */
 tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor router, tlhip_tensor gate, tlhip_tensor up,
                        tlhip_tensor down, int top_k, int normalize, tlhip_tensor y);
 

@@ -14,7 +14,8 @@ extern "C" tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits,
     if (logits->ndim != 1 && logits->ndim != 2)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: expects [V] or [rows, V] logits, got %s", op, shape_str(logits).c_str());
     const int64_t V = last_dim(logits), rows = logits->ndim == 2 ? logits->shape[0] : 1;
-    if (V < 1 || V > (1 << 30) || rows > INT32_MAX)
+    // (a launch holds fewer than 2^32 threads, and a row takes 256 at least)
+    if (V < 1 || V > (1 << 30) || rows >= (1 << 24))
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: logits %s", op, shape_str(logits).c_str());
     if (n_top < 0 || n_top > kMaxTop || n_top > V)
         return fail(TLHIP_ERR_INVALID_DIMENSION, "%s: n_top %d not in 0..min(%d, %lld)", op, n_top, kMaxTop, (long long)V);

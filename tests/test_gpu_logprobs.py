@@ -139,3 +139,18 @@ def test_refusals(dev):
     assert kind(lambda: token_logprobs(x, dev.empty((3,), F32))) == "DtypeError"
     assert kind(lambda: token_logprobs(dev.empty((3, 100), I32), ids)) == "DtypeError"
     assert kind(lambda: token_logprobs(dev.empty((3, 96), Q8_0), ids)) == "DtypeError"
+    big = dev.empty((2 ** 24, 1))
+    assert kind(lambda: token_logprobs(big)) == "InvalidDimension"
+
+
+def test_most_rows(dev):
+    """The largest launch there is: rows of one token, whose probability is 1."""
+    n = 2 ** 24 - 1
+    x = dev.tensor(np.tile(np.array([[3.0], [-65504.0], [np.nan]], np.float16), (n // 3, 1)))
+    h = token_logprobs(x)[1].numpy()
+    # not 0: the sums are in reference to a rounded m log2(e), so z = 2^d and t
+    # = d 2^d with a |d| of up to half a step of it, and H = log z - t / z
+    # keeps the roundings of 2^d, of the logarithm and of the quotient, each of
+    # numbers near 1 or 0: reference()'s bound at V = 1, x = m
+    tol = U * (1 / 64 + 64) * 2
+    assert (np.abs(h[0::3]) <= tol).all() and (np.abs(h[1::3]) <= tol).all() and np.isnan(h[2::3]).all()
