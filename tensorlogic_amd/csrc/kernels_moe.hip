@@ -36,14 +36,18 @@ namespace tlhip {
 
 namespace {
 
-constexpr int kWaves = 4;                  // of a workgroup of the products
 constexpr int kTokens = 256;               // tokens of one round of launches (moe.cpp)
-// Slots of weights that a wave has in flight, and the columns staged in LDS at a
-// time (or one round of slots, if that is more): two workgroups fit on a CU with
-// rows of 5632.  (Deeper rings and more columns measured the same; with one
-// workgroup to a CU 13 tokens' down took 45 us instead of 33.)
+// Waves of a workgroup of the products, slots of weights that a wave has in
+// flight, and the columns staged in LDS at a time (or one round of slots, if
+// that is more): two workgroups fit on a CU with rows of 5632.  (Deeper rings
+// and, for gate and up, more columns or waves measured the same or less.)
+// Down's columns are f32, to be split in two, so with several tokens to an
+// expert eight waves share them: 13 tokens of 8 Q8_0 experts 2048 x 5632, two
+// each, 27 us against 33, 30 tokens of 4096 x 5632 12 us less; five tokens of
+// 64 experts, six each, are 5 us faster with four.
 constexpr int kRing = 2;
-constexpr int kColumnBytes = 24 << 10;
+constexpr int kWaves = 4, kColumnBytes = 24 << 10;
+constexpr int kDownWaves = 8, kDownColumnBytes = 48 << 10;
 
 // ---------------------------------------------------------------------------
 // router
@@ -313,7 +317,7 @@ __device__ __forceinline__ f4 low_part(const f4& p) {
     for (int k = 0; k < 4; k++) r[k] = p[k] - (float)(h16)p[k];
     return r;
 }
-template <typename LOADER>
+template <typename LOADER, int NW>
 struct Stage : LOADER {
     struct Ahead {
         typename LOADER::Run p[kPieces], q[kPieces];
@@ -323,7 +327,7 @@ struct Stage : LOADER {
         const uint32_t by_nt = 0xFFFFFFFFu / this->nt + 1;   // i / nt = umulhi(i, by_nt): i nt < 2^32
 #pragma unroll
         for (int k = 0; k < kPieces; k++) {
-            const int i = i0 + k * kWaves * 64, bs = this->nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * this->nt, b = c0 + (bs >> 2);
+            const int i = i0 + k * NW * 64, bs = this->nt == 1 ? i : (int)__umulhi(i, by_nt), t = i - bs * this->nt, b = c0 + (bs >> 2);
             v.p[k] = v.q[k] = typename LOADER::Run{};
             if (i < blocks * 4 * this->nt && b < nb) this->get(v.p[k], v.q[k], t, b, bs & 3);
         }
@@ -331,12 +335,12 @@ struct Stage : LOADER {
     __device__ __forceinline__ void store(const Ahead& v, int i0, h8* cols, int blocks) const {
 #pragma unroll
         for (int k = 0; k < kPieces; k++)
-            if (i0 + k * kWaves * 64 < blocks * 4 * this->nt) this->set(v.p[k], v.q[k], cols, i0 + k * kWaves * 64);
+            if (i0 + k * NW * 64 < blocks * 4 * this->nt) this->set(v.p[k], v.q[k], cols, i0 + k * NW * 64);
     }
     __device__ __forceinline__ void fetch(Ahead& v, int c0, int blocks, int nb) const { load(v, threadIdx.x, c0, blocks, nb); }
     __device__ __forceinline__ void put(Ahead& v, h8* cols, int c0, int blocks, int nb) const {
         store(v, threadIdx.x, cols, blocks);
-        for (int i0 = threadIdx.x + kPieces * kWaves * 64; i0 < blocks * 4 * this->nt; i0 += kPieces * kWaves * 64) {
+        for (int i0 = threadIdx.x + kPieces * NW * 64; i0 < blocks * 4 * this->nt; i0 += kPieces * NW * 64) {
             load(v, i0, c0, blocks, nb);
             store(v, i0, cols, blocks);
         }
@@ -382,17 +386,18 @@ struct LoadH {
 struct Layout {
     int column_bytes, ring_at, scales_at, bytes;
 };
-constexpr int kRedBytes = kWaves * 4 * 64 * 16;   // the waves' sums, in place of columns and ring at the end
-template <int WT, int NR, int KS>
+template <int WT, int NR, int KS, int NW>
 __host__ __device__ inline Layout layout(int nb, int max_cols) {
     constexpr int round = Slot<WT>::BLOCKS * KS;
     Layout l;
     const int whole = (nb + round - 1) / round * round * 64 * max_cols, least = round * 64 * max_cols;
-    l.column_bytes = whole < kColumnBytes ? whole : kColumnBytes > least ? kColumnBytes : least;
+    constexpr int want = NW == kWaves ? kColumnBytes : kDownColumnBytes;
+    l.column_bytes = whole < want ? whole : want > least ? want : least;
     l.ring_at = l.column_bytes;
-    l.scales_at = l.ring_at + kWaves * NR * kRing * Slot<WT>::BYTES;
-    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : kWaves / KS * NR * scale_bytes(nb));
-    if (KS > 1 && l.bytes < kRedBytes) l.bytes = kRedBytes;
+    l.scales_at = l.ring_at + NW * NR * kRing * Slot<WT>::BYTES;
+    l.bytes = l.scales_at + (WT == TLHIP_F16 ? 0 : NW / KS * NR * scale_bytes(nb));
+    constexpr int red = NW * 4 * 64 * 16;   // the waves' sums, in place of columns and ring at the end
+    if (KS > 1 && l.bytes < red) l.bytes = red;
     return l;
 }
 
@@ -514,7 +519,7 @@ template <int WT, int CT, int KS, bool ONE>
 __device__ __forceinline__ void gate_up_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds,
                                              MoeShared& sh, int one_pair = 0) {
     f4 acc[2][CT];
-    const Stage<LoadX<WT, ONE>> stage{{a, sh.list + t0, nt}};
+    const Stage<LoadX<WT, ONE>, kWaves> stage{{a, sh.list + t0, nt}};
     const int tiles = a.I / 16, nb = a.K / 32;
     // (a wave past the last tile computes that one and stores nothing)
     const size_t row = (size_t)e * a.I + 16 * (tile < tiles ? tile : tiles - 1);
@@ -573,10 +578,10 @@ __device__ __forceinline__ float scale_for(float m) {
 
 // Down: 16 rows of one expert; the columns are the hi and lo parts of each
 // token's h, one after the other.
-template <int WT, int CT, int KS>
+template <int WT, int CT, int KS, int NW>
 __device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int tile, int t0, int nt, const Layout& at, uint8_t* lds, MoeShared& sh) {
     f4 acc[1][CT];
-    const Stage<LoadH<WT>> stage{{a, sh.list + t0, nt, sh.scale + t0}};
+    const Stage<LoadH<WT>, NW> stage{{a, sh.list + t0, nt, sh.scale + t0}};
     const int tiles = a.K / 16, nb = a.I / 32;
     const size_t row = (size_t)e * a.K + 16 * (tile < tiles ? tile : tiles - 1);
     const Rows<WT> w[1] = {Rows<WT>(a.down, row, nb)};
@@ -596,17 +601,17 @@ __device__ __forceinline__ void down_tile(const MoeArgs& a, int e, int tile, int
     }
 }
 
-template <int WT, int KS, int CT>
-__global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a, Layout at) {
+template <int WT, int KS, int CT, int NW>
+__global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a, Layout at) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeShared sh;
-    constexpr int TW = kWaves / KS;
+    constexpr int TW = NW / KS;
     const int groups = (a.K / 16 + TW - 1) / TW;
     const int tile = (int)(blockIdx.x % groups) * TW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / KS;
     const int e = __builtin_amdgcn_readfirstlane(slot_expert(a, blockIdx.x / groups, sh));
     if (e < 0) return;
     const int count = sh.count, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int t = wave; t < count; t += kWaves) {
+    for (int t = wave; t < count; t += NW) {
         const float* hm = a.hmax + (size_t)sh.list[t] * (a.I / 16);
         float m = 0.0f;
         for (int i = lane; i < a.I / 16; i += 64) m = fmaxf(m, hm[i]);
@@ -616,8 +621,8 @@ __global__ __launch_bounds__(kWaves * 64) void moe_down_kernel(MoeArgs a, Layout
     __syncthreads();
     for (int t0 = 0; t0 < count; t0 += 8 * CT) {
         const int nt = count - t0 < 8 * CT ? count - t0 : 8 * CT;
-        if (CT == 1 || nt <= 8) down_tile<WT, 1, KS>(a, e, tile, t0, nt, at, lds, sh);
-        else down_tile<WT, CT, KS>(a, e, tile, t0, nt, at, lds, sh);
+        if (CT == 1 || nt <= 8) down_tile<WT, 1, KS, NW>(a, e, tile, t0, nt, at, lds, sh);
+        else down_tile<WT, CT, KS, NW>(a, e, tile, t0, nt, at, lds, sh);
         __syncthreads();
     }
 }
@@ -754,40 +759,48 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
 constexpr int kLdsDynamic = 156 << 10;
 static_assert(kLdsDynamic + sizeof(MoeShared) <= 160 << 10, "LDS of a CU");
 static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "rows of a Q type fit");
-static_assert((32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
+static_assert(kDownColumnBytes + (64 << 10) <= kLdsDynamic && (32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
 
 // Up to 16 (down: 8) tokens, no expert has more columns than one B operand holds.
 template <int WT, int KS>
 void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
     const unsigned grid = slots * ((a.I / 16 + kWaves / KS - 1) / (kWaves / KS));
-    const Layout at = layout<WT, 2, KS>(a.K / 32, a.M < 32 ? a.M : 32);
+    const Layout at = layout<WT, 2, KS, kWaves>(a.K / 32, a.M < 32 ? a.M : 32);
     if (a.M == 1) moe_gate_up_kernel<WT, KS, 1, true><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     else if (a.M <= 16) moe_gate_up_kernel<WT, KS, 1, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     else moe_gate_up_kernel<WT, KS, 2, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
 }
-template <int WT, int KS>
+template <int WT, int KS, int NW>
 void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    const unsigned grid = slots * ((a.K / 16 + kWaves / KS - 1) / (kWaves / KS));
-    const Layout at = layout<WT, 1, KS>(a.I / 32, a.M < 16 ? 2 * a.M : 32);
-    if (a.M <= 8) moe_down_kernel<WT, KS, 1><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
-    else moe_down_kernel<WT, KS, 2><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
+    const unsigned grid = slots * ((a.K / 16 + NW / KS - 1) / (NW / KS));
+    const Layout at = layout<WT, 1, KS, NW>(a.I / 32, a.M < 16 ? 2 * a.M : 32);
+    if (a.M <= 8) moe_down_kernel<WT, KS, 1, NW><<<grid, NW * 64, at.bytes, s>>>(a, at);
+    else moe_down_kernel<WT, KS, 2, NW><<<grid, NW * 64, at.bytes, s>>>(a, at);
     moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
 }
 // Waves that share out the k of a tile of 16 rows: as few as leave two
 // workgroups of four waves for every CU (the more tiles a workgroup has, the
 // fewer times the columns are staged), and no fewer than LDS has room for.
-template <int WT, int NR>
+template <int WT, int NR, int NW>
 int waves_of_tile(int64_t tiles, int nb) {
-    if (tiles >= 2048 && layout<WT, NR, 1>(nb, 32).bytes <= kLdsDynamic) return 1;
-    if (tiles >= 1024 && layout<WT, NR, 2>(nb, 32).bytes <= kLdsDynamic) return 2;
+    if (tiles >= 2048 && layout<WT, NR, 1, NW>(nb, 32).bytes <= kLdsDynamic) return 1;
+    if (tiles >= 1024 && layout<WT, NR, 2, NW>(nb, 32).bytes <= kLdsDynamic) return 2;
     return 4;
 }
 template <int WT>
 void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    switch (waves_of_tile<WT, 2>((int64_t)slots * (a.I / 16), a.K / 32)) {
+    switch (waves_of_tile<WT, 2, kWaves>((int64_t)slots * (a.I / 16), a.K / 32)) {
         case 1: return gate_up<WT, 1>(s, a, slots);
         case 2: return gate_up<WT, 2>(s, a, slots);
         default: return gate_up<WT, 4>(s, a, slots);
+    }
+}
+template <int WT, int NW>
+void down_waves(hipStream_t s, const MoeArgs& a, unsigned slots) {
+    switch (waves_of_tile<WT, 1, NW>((int64_t)slots * (a.K / 16), a.I / 32)) {
+        case 1: return down<WT, 1, NW>(s, a, slots);
+        case 2: return down<WT, 2, NW>(s, a, slots);
+        default: return down<WT, 4, NW>(s, a, slots);
     }
 }
 template <int WT>
@@ -799,11 +812,8 @@ void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
             return;
         }
     }
-    switch (waves_of_tile<WT, 1>((int64_t)slots * (a.K / 16), a.I / 32)) {
-        case 1: return down<WT, 1>(s, a, slots);
-        case 2: return down<WT, 2>(s, a, slots);
-        default: return down<WT, 4>(s, a, slots);
-    }
+    if (a.M * a.top >= 2 * a.E) down_waves<WT, kDownWaves>(s, a, slots);
+    else down_waves<WT, kWaves>(s, a, slots);
 }
 
 }  // namespace
