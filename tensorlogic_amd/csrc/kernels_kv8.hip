@@ -69,8 +69,13 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
     // the tile in LDS, 16 bytes between every 256: neighbouring lanes' pieces
     // lie 256 bytes apart in it and would share their banks
     auto lds = [](int at) { return at + (at >> 8) * 16; };
-    const int is_v = blockIdx.x & 1;
-    const int head = (blockIdx.x >> 1) % p.n_kv, unit = (blockIdx.x >> 1) / p.n_kv;
+    // Workgroups go round the eight XCDs; the heads of a unit, whose rows share
+    // cache lines, stay on one of them when there are enough units.
+    const int items = 2 * p.n_kv, units = p.n_full + ((p.len0 + p.S) & 31 ? 1 : 0);
+    const int j = units >= 8 ? blockIdx.x >> 3 : blockIdx.x, item = j % items;
+    const int unit = units >= 8 ? j / items * 8 + (blockIdx.x & 7) : j / items;
+    if (unit >= units) return;
+    const int is_v = item >= p.n_kv, head = is_v ? item - p.n_kv : item;
     const int tid = threadIdx.x;
     const size_t row = (size_t)p.n_kv * D;
     const uint16_t* src = (is_v ? p.v : p.k) + (size_t)head * D;
@@ -613,7 +618,7 @@ tlhip_status launch_kv8_write(hipStream_t s, const Kv8Write& p) {
     const int end = p.len0 + p.S;
     const int units = p.n_full + ((end & 31) ? 1 : 0);
     if (units == 0) return TLHIP_OK;
-    const dim3 grid((unsigned)units * p.n_kv * 2);
+    const dim3 grid((unsigned)(units >= 8 ? (units + 7) / 8 * 8 : units) * p.n_kv * 2);
 #define CALL(D) kv8_write_kernel<D><<<grid, 256, 0, s>>>(p)
     KV8_DISPATCH(p.D, CALL)
 #undef CALL
