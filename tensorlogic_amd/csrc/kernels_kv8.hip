@@ -53,18 +53,21 @@ __device__ __forceinline__ float abs_max8(const h8& v, float m) {
     return m;
 }
 
-// One workgroup of 256 threads per (unit, KV head, K or V).  Units 0 ..
-// n_full - 1 are the blocks that this call completes: their positions come
-// from the old tail (before len0) and the new rows.  The last unit, when
-// rows are left over, writes them to the new tail.  Old and new tail are the
-// same buffer only if no block is completed, so nothing is written that
-// another workgroup reads.  Bound by launch and load latency below about 500
-// rows, then by memory.
+// A workgroup per (unit, KV head, K or V).  Units 0 .. n_full - 1 are the
+// blocks that this call completes: their positions come from the old tail
+// (before len0) and the new rows.  The last unit, when rows are left over,
+// writes them to the new tail.  Old and new tail are the same buffer only if
+// no block is completed, so nothing is written that another workgroup reads.
+// Bound by launch and latency below about 1000 rows (46 rows of 4 heads of 64:
+// 3.6 us a call), then by memory (2048 rows of 32 heads of 80, 31 MB: 9.6 us,
+// 3.3 TB/s; with 256 threads 10.0).
+constexpr int kWriteThreads = 128;
 template <int D>
-__global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
+__global__ __launch_bounds__(kWriteThreads) void kv8_write_kernel(Kv8Write p) {
     constexpr int PIECES = 4 * D;            // 8 values each
-    constexpr int PT = (PIECES + 255) / 256; // pieces of a thread
-    __shared__ float red[4];
+    constexpr int PT = (PIECES + kWriteThreads - 1) / kWriteThreads; // pieces of a thread
+    __shared__ float red[kWriteThreads / 64];
+    __shared__ int bad_row[32];
     __shared__ __align__(16) uint8_t tile[34 * D];
     // the tile in LDS, 16 bytes between every 256: neighbouring lanes' pieces
     // lie 256 bytes apart in it and would share their banks
@@ -79,74 +82,79 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
     const int tid = threadIdx.x;
     const size_t row = (size_t)p.n_kv * D;
     const uint16_t* src = (is_v ? p.v : p.k) + (size_t)head * D;
-    const int b0 = p.len0 >> 5;
+    const int block = (p.len0 >> 5) + unit, old = p.len0 - block * 32;   // keys below old are in the tail
 
-    if (unit == p.n_full) {   // the rows left over: positions first .. len0 + S - 1
-        const int first = p.n_full ? (b0 + p.n_full) * 32 : p.len0;
-        const int end = p.len0 + p.S - (first & ~31);   // rows the tail holds then
-        uint16_t* t = (is_v ? p.tail_v : p.tail_k) + ((size_t)p.tail_dst * p.n_kv + head) * 32 * D;
-        // a fresh tail is cleared past its rows: attention reads whole tiles
-        const int r0 = first & 31, r1 = r0 == 0 ? 32 : end;
-        for (int r = r0 + (tid >> 6); r < r1; r += 4) {
-            const int lane = tid & 63;
-            const bool have = r < end;
-            float bad = 0.0f;
-            if (is_v && have)
-                for (int u = lane; u < D / 8; u += 64) {
-                    const h8 x = *(const h8*)(src + (size_t)((first & ~31) + r - p.len0) * row + 8 * u);
-                    bad = abs_max8(x, bad);
-                }
-            const bool nan = is_v && __any(bad == INFINITY);
-            for (int u = lane; u < D / 8; u += 64) {
-                h8 x = {};
-                if (have && !nan) x = *(const h8*)(src + (size_t)((first & ~31) + r - p.len0) * row + 8 * u);
-                if (is_v) {
+    // The block's new rows, 8 values a piece (no branch among the loads: each
+    // would wait for those before it); past the last row, or before the first,
+    // that one again.
+    h8 x[PT];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const h16 e = x[i];   // (a bit cast of the vector's element itself takes element 0)
-                        t[v_at(r, 8 * u + i)] = __builtin_bit_cast(uint16_t, e);
-                    }
-                } else {
-                    *(h8*)(t + k_at(r, 8 * u)) = x;
-                }
+    for (int j = 0; j < PT; j++) {
+        const int i = min(tid + kWriteThreads * j, PIECES - 1), key = i / (D / 8), u = i % (D / 8);
+        x[j] = *(const h8*)(src + (size_t)min(max(key - old, 0), p.S - 1) * row + 8 * u);
+    }
+
+    if (unit == p.n_full) {   // the rows left over
+        // a fresh tail is cleared past its rows: attention reads whole tiles
+        const int end = p.len0 + p.S - block * 32, r0 = max(old, 0), r1 = r0 == 0 ? 32 : end;
+        const size_t th = (size_t)p.tail_dst * p.n_kv + head;
+        uint16_t* t = (is_v ? p.tail_v : p.tail_k) + th * 32 * D;
+        if (is_v) {
+            if (tid < 32) bad_row[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PT; j++) {
+                const int key = min(tid + kWriteThreads * j, PIECES - 1) / (D / 8);
+                if (key >= r0 && key < end && abs_max8(x[j], 0.0f) == INFINITY) bad_row[key] = 1;
             }
-            if (is_v && lane == 0)
-                p.tail_flag[((size_t)p.tail_dst * p.n_kv + head) * 32 + r] = nan ? NAN : 0.0f;
+            __syncthreads();
+            if (tid >= r0 && tid < r1) p.tail_flag[th * 32 + tid] = bad_row[tid] ? NAN : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < PT; j++) {
+            const int i = tid + kWriteThreads * j, key = i / (D / 8), u = i % (D / 8);
+            if (key < r0 || key >= r1) continue;
+            if (key >= end || (is_v && bad_row[key])) x[j] = h8{};
+            if (is_v) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const h16 v = x[j][e];   // (a bit cast of the vector's element itself takes element 0)
+                    t[v_at(key, 8 * u + e)] = __builtin_bit_cast(uint16_t, v);
+                }
+            } else {
+                *(h8*)(t + k_at(key, 8 * u)) = x[j];
+            }
         }
         return;
     }
 
-    const int block = b0 + unit;
-    h8 x[PT];
     float m = 0.0f;
+    if (old > 0) {   // its first rows are in the tail
+        const size_t th = (size_t)p.tail_src * p.n_kv + head;
+        const uint16_t* t = (is_v ? p.tail_v : p.tail_k) + th * 32 * D;
+        if (is_v && tid < old && p.tail_flag[th * 32 + tid] != 0.0f) m = INFINITY;
 #pragma unroll
-    for (int j = 0; j < PT; j++) {
-        const int i = tid + 256 * j, key = i / (D / 8), u = i % (D / 8);
-        x[j] = h8{};
-        if (i >= PIECES) continue;
-        const int pos = block * 32 + key;
-        if (pos >= p.len0) {
-            x[j] = *(const h8*)(src + (size_t)(pos - p.len0) * row + 8 * u);
-        } else {   // from the tail
-            const size_t th = (size_t)p.tail_src * p.n_kv + head;
-            const uint16_t* t = (is_v ? p.tail_v : p.tail_k) + th * 32 * D;
+        for (int j = 0; j < PT; j++) {
+            const int i = min(tid + kWriteThreads * j, PIECES - 1), key = i / (D / 8), u = i % (D / 8);
+            h8 y;
             if (is_v) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[j][e] = __builtin_bit_cast(h16, t[v_at(key, 8 * u + e)]);
-                if (p.tail_flag[th * 32 + key] != 0.0f) m = INFINITY;
+                for (int e = 0; e < 8; e++) y[e] = __builtin_bit_cast(h16, t[v_at(key, 8 * u + e)]);
             } else {
-                x[j] = *(const h8*)(t + k_at(key, 8 * u));
+                y = *(const h8*)(t + k_at(key, 8 * u));
             }
+            x[j] = key < old ? y : x[j];
         }
-        m = abs_max8(x[j], m);
     }
-    m = block_max1<4>(m, red);
+#pragma unroll
+    for (int j = 0; j < PT; j++) m = abs_max8(x[j], m);
+    m = block_max1<kWriteThreads / 64>(m, red);
     const bool bad = m == INFINITY;
     const float inv = m > 0.0f && !bad ? 127.0f / m : 0.0f;
     const float scale = bad ? NAN : m > 0.0f ? m / 127.0f : 1.0f;
 #pragma unroll
     for (int j = 0; j < PT; j++) {
-        const int i = tid + 256 * j, key = i / (D / 8), u = i % (D / 8);
+        const int i = tid + kWriteThreads * j, key = i / (D / 8), u = i % (D / 8);
         if (i >= PIECES) continue;
         uint8_t q[8];
 #pragma unroll
@@ -167,7 +175,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write p) {
     __syncthreads();
     const size_t bt = (size_t)head * p.n_blocks + block;
     uint8_t* dst = (is_v ? p.vq : p.kq) + bt * 32 * D;
-    for (int i = tid; i < 2 * D; i += 256) *(u4*)(dst + 16 * i) = *(const u4*)(tile + lds(16 * i));
+    for (int i = tid; i < 2 * D; i += kWriteThreads) *(u4*)(dst + 16 * i) = *(const u4*)(tile + lds(16 * i));
     if (tid == 0) (is_v ? p.vs : p.ks)[bt] = scale;
 }
 
@@ -617,9 +625,9 @@ bool kv8_head_dim_ok(int D) { return D == 32 || D == 64 || D == 80 || D == 96 ||
 tlhip_status launch_kv8_write(hipStream_t s, const Kv8Write& p) {
     const int end = p.len0 + p.S;
     const int units = p.n_full + ((end & 31) ? 1 : 0);
-    if (units == 0) return TLHIP_OK;
+    if (units == 0 || p.S == 0) return TLHIP_OK;
     const dim3 grid((unsigned)(units >= 8 ? (units + 7) / 8 * 8 : units) * p.n_kv * 2);
-#define CALL(D) kv8_write_kernel<D><<<grid, 256, 0, s>>>(p)
+#define CALL(D) kv8_write_kernel<D><<<grid, kWriteThreads, 0, s>>>(p)
     KV8_DISPATCH(p.D, CALL)
 #undef CALL
     return TLHIP_OK;
