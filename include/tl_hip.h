@@ -330,11 +330,12 @@ tlhip_status tlhip_kvcache_create_f32(tlhip_ctx ctx, int n_layers, int max_ctx, 
  * in f16 (later appends do not change it); the attention entry points read
  * the int8 values with their scales, unrounded, and keep scores, weights and
  * sums in f32 (the scale argument is not rounded to f16, and a position a
- * query does not see weighs nothing).  K and V should be finite: a block
- * (past the last whole one: a row) of a head that holds an infinity or NaN
- * shows as NaN to the queries that see it.  head_dim 32, 64, 80, 96, 128 or
- * 256, at most 1024 KV heads; used on the context it was created on only
- * (else InvalidArgument).                                                  */
+ * query does not see weighs nothing).  K and V should be finite: a block of
+ * a head that holds an infinity or NaN (past the last whole block: a row of
+ * V that does; a row of K scores as f16 arithmetic has it) shows as NaN to
+ * the queries that see it.  head_dim 32, 64, 80, 96, 128 or 256, at most
+ * 1024 KV heads; used on the context it was created on only (else
+ * InvalidArgument).                                                        */
 tlhip_status tlhip_kvcache_create_q8(tlhip_ctx ctx, int n_layers, int max_ctx, int n_kv_heads,
                                      int head_dim, tlhip_kvcache* out);
 tlhip_status tlhip_kvcache_free(tlhip_kvcache c);

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kWriteThreads) void kv8_write_kernel(Kv8Write p) {
     m = block_max1<kWriteThreads / 64>(m, red);
     const bool bad = m == INFINITY;
     const float inv = m > 0.0f && !bad ? 127.0f / m : 0.0f;
-    const float scale = bad ? NAN : m > 0.0f ? m / 127.0f : 1.0f;
+    const float scale = bad ? NAN : m / 127.0f;
 #pragma unroll
     for (int j = 0; j < PT; j++) {
         const int i = tid + kWriteThreads * j, key = i / (D / 8), u = i % (D / 8);
@@ -224,14 +224,16 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read p) {
 // these are the 8 keys that it supplies to the second product as B, so the
 // probabilities never leave the lane (the V tile's key order sees to it).
 //
-// Scales: with x_j = scale * log2(e) * ks_b * (q . kq_j) + log2(vs_b) and M a
-// running bound of x, the weights w_j = 2^(x_j - M) carry V's scale already:
-//   o = sum_j w_j vq_j / sum_j (w_j / vs_b).
-// So the f16 operand P is the weight that multiplies the bytes, near 1 where
-// it matters whatever the scales are.  M is raised when a row's largest x
-// passes it by more than 8: P stays below 2^8 and most tiles rescale nothing.
-// Scores, weights, sums and O are f32; P's rounding to f16 (2^-11 relative,
-// for the matrix cores) is the only one before the result's.
+// Scales: with x_j = scale * log2(e) * ks_b * (q . kq_j), M a running bound of
+// x and C a power of two near the blocks' scales of V, the weights
+//   w_j = 2^(x_j - M) vs_b / C
+// carry V's scale already:  o = C sum_j w_j vq_j / sum_j (w_j C / vs_b).
+// M is raised when a row's largest x passes it by more than 8, C moved (and O
+// with it, exactly) when a block's scale is not within C / 2 .. 64 C: so the
+// f16 operand P = w stays below 2^14, most tiles rescale nothing, and a weight
+// loses bits to f16's range only below 2^-13 of the row's largest.  Scores,
+// weights, sums and O are f32; P's rounding to f16 (2^-11 relative, for the
+// matrix cores) is the only one before the result's.
 constexpr float kLog2e = 1.44269504088896f;
 constexpr float kNone = -3.0e38f;   // M before any key
 
@@ -262,6 +264,7 @@ struct Kv8Wave {
     int pos[NQ];
     int c16, g;
     float sl;             // |scale| * log2(e) (the queries carry its sign)
+    uint32_t C;           // the unit of o, a power of two, as the bits of an f32
 
     static __device__ __forceinline__ bool chunk_ok(int c, int g) { return D % 32 == 0 || c < NC - 1 || g < 2; }
     static __device__ __forceinline__ bool dim_ok(int p, int c16) { return D % 32 == 0 || p < NC - 1 || c16 < 8; }
@@ -271,6 +274,7 @@ struct Kv8Wave {
         c16 = lane & 15;
         g = lane >> 4;
         sl = fabsf(p.scale) * kLog2e;
+        C = 0x3F800000u;
         const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
@@ -292,13 +296,13 @@ struct Kv8Wave {
     }
 
     // One tile: kx(c, t) the lane's keys (8 dims of chunk c of key 2 c16 + t),
-    // vx(t) its V^T rows; f: the factor of the score; lv(i): log2 of V's scale
-    // at the lane's key i (8g + 2 (i & 3) + (i >> 2)); iv: 1 / that scale.
+    // vx(t) its V^T rows; f: the factor of the score; scale: of V.  TAIL: scale
+    // 1 = C, and flag(i) of the lane's key i (8g + 2 (i & 3) + (i >> 2)).
     // Per score a maximum (two to an instruction), one fused operation, one
     // exp and half a conversion; the weights' sum comes from the matrix cores
     // (a row of ones), so that it is the sum of the weights as rounded.
-    template <bool MASK, bool EACH, typename KX, typename VX, typename LV>
-    __device__ __forceinline__ void tile(const KX& kx, const VX& vx, float f, const LV& lv, float iv, int key0) {
+    template <bool MASK, bool TAIL, typename KX, typename VX, typename FLAG>
+    __device__ __forceinline__ void tile(const KX& kx, const VX& vx, float f, float scale, const FLAG& flag, int key0) {
         f32x4 sc[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; n++) sc[n][0] = sc[n][1] = f32x4{0, 0, 0, 0};
@@ -318,14 +322,23 @@ struct Kv8Wave {
         for (int n = 0; n < NQ; n++) {
             float m = kNone;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = EACH ? fmaf(sc[n][i >> 2][i & 3], f, lv(i)) : sc[n][i >> 2][i & 3];
-                m = fmaxf(m, seen(n, i) ? x : kNone);
-            }
-            top[n] = EACH ? m : fmaf(m, f, lv(0));
+            for (int i = 0; i < 8; i++) m = fmaxf(m, seen(n, i) ? sc[n][i >> 2][i & 3] : kNone);
+            top[n] = m * f;
             higher |= top[n] > M[n] + 8.0f;
         }
+        float ratio = scale * __uint_as_float(0x7F000000u - C), lv = __builtin_amdgcn_logf(ratio), iv = __builtin_amdgcn_rcpf(ratio);
+        if constexpr (!TAIL) higher |= !fits(__float_as_uint(scale) >> 23, C);
         if (__any(higher)) {
+            if constexpr (!TAIL) {
+                const uint32_t e = __builtin_amdgcn_readfirstlane(__float_as_uint(scale)) >> 23;
+                if (!fits(e, C)) {
+                    // (a block of zeros: any scale; a NaN: for the keys that are seen)
+                    if (e - 1 < 254) unit(e << 23);
+                    ratio = e - 1 < 254 ? scale * __uint_as_float(0x7F000000u - C) : 1.0f;
+                    lv = e == 255 ? NAN : __builtin_amdgcn_logf(ratio);
+                    iv = __builtin_amdgcn_rcpf(ratio);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
                 const float m = rows4_max(top[n]), mn = m > M[n] + 8.0f ? m : M[n], r = __builtin_amdgcn_exp2f(M[n] - mn);
@@ -338,10 +351,10 @@ struct Kv8Wave {
         h8 pr[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-            const float c = EACH ? -M[n] : lv(0) - M[n];
+            const float c = TAIL ? -M[n] : lv - M[n];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float x = fmaf(sc[n][i >> 2][i & 3], f, EACH ? lv(i) + c : c);
+                const float x = fmaf(sc[n][i >> 2][i & 3], f, TAIL ? flag(i) + c : c);
                 pr[n][i] = (h16)__builtin_amdgcn_exp2f(seen(n, i) ? x : -INFINITY);
             }
         }
@@ -349,7 +362,7 @@ struct Kv8Wave {
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
             const f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pr[n], f32x4{0, 0, 0, 0}, 0, 0, 0);
-            l[n] = fmaf(s[0], iv, l[n]);
+            l[n] = TAIL ? l[n] + s[0] : fmaf(s[0], iv, l[n]);
         }
 #pragma unroll
         for (int t = 0; t < 2 * NC; t++) {
@@ -357,6 +370,18 @@ struct Kv8Wave {
 #pragma unroll
             for (int n = 0; n < NQ; n++) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pr[n], o[n][t], 0, 0, 0);
         }
+    }
+
+    // Whether a scale of exponent bits e lies within C / 2 .. 64 C.
+    static __device__ __forceinline__ bool fits(uint32_t e, uint32_t C) { return e - (C >> 23) + 1 <= 6u; }
+    // Moves C to another power of two, and o with it.
+    __device__ __forceinline__ void unit(uint32_t to) {
+        const float r = __uint_as_float(C) * __uint_as_float(0x7F000000u - to);
+        C = to;
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int t = 0; t < 2 * NC; t++) o[n][t] *= r;
     }
 
     // Tiles t0, t0 + step, ... below t1 (tile nfull, if among them, is the
@@ -390,24 +415,26 @@ struct Kv8Wave {
                 kc[c] = kr[c];
                 vc[c] = vr[c];
             }
-            const float f = sl * fk, lv = __builtin_amdgcn_logf(fv), iv = __builtin_amdgcn_rcpf(fv);
+            const float f = sl * fk;
+            const float scale = fv;
             if (next < tq) load(next);
             tile<decltype(mask)::value, false>([&](int c, int h) { return bytes_h8(kc[c][2 * h], kc[c][2 * h + 1]); },
                                                [&](int h) { return bytes_h8(vc[h >> 1][2 * (h & 1)], vc[h >> 1][2 * (h & 1) + 1]); }, f,
-                                               [&](int) { return lv; }, iv, 32 * b);
+                                               scale, [](int) { return 0.0f; }, 32 * b);
         };
         if (t < tq) load(t);
         const int whole = (pos0 + 1) >> 5;   // tiles below it are seen by every row
         for (; t < tq && t < whole; t += step) step_over(std::false_type{}, t, t + step);
         for (; t < tq; t += step) step_over(std::true_type{}, t, t + step);
+        unit(0x3F800000u);
         if (t < t1) {   // the tail: f16 values
             const size_t th = (size_t)p.tail_cur * p.n_kv + head;
             const uint16_t* kt = p.tail_k + th * 32 * D;
             const uint16_t* vt = p.tail_v + th * 32 * D;
             const float* fl = p.tail_flag + th * 32 + 8 * g;
-            float lv[8];
+            float flag[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) lv[i] = fl[2 * (i & 3) + (i >> 2)];
+            for (int i = 0; i < 8; i++) flag[i] = fl[2 * (i & 3) + (i >> 2)];
             tile<true, true>(
                 [&](int c, int h) {
                     h8 a = {};
@@ -419,7 +446,7 @@ struct Kv8Wave {
                     if (dim_ok(h >> 1, c16)) a = *(const h8*)(vt + ((((h >> 1) * 16 + c16) * 4 + g) * 2 + (h & 1)) * 8);
                     return a;
                 },
-                sl, [&](int i) { return lv[i]; }, 1.0f, 32 * t);
+                sl, 1.0f, [&](int i) { return flag[i]; }, 32 * t);
         }
     }
 

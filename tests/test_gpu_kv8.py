@@ -188,6 +188,53 @@ def test_non_finite_values_stay_where_they_are_seen(dev, bad):
     assert np.isnan(c.get_v(0).numpy()[64:96, 2]).all() and np.isfinite(c.get_v(0).numpy()[:, 3]).all()
 
 
+@pytest.mark.parametrize("S,past", [(70, 30), (9, 25)])
+def test_rows_before_a_bad_block_in_one_tile_of_rows(dev, S, past):
+    """Queries on both sides of a block's start: those before it see nothing of its NaN."""
+    n = S + past
+    for which in (0, 1):
+        kv = list(rows(11, n, 1, 64))
+        kv[which][33, 0, 5] = np.nan if n < 64 else np.inf   # (in f16 still, an infinite key's score is what it is)
+        kv[0][:32] = kv[0][:32] / 8
+        q = np.random.default_rng(11).standard_normal((S, 2, 64)).astype(np.float16)
+        c = KVCache(dev, 1, 128, 1, 64, Q8_0)
+        c.set(0, dev.tensor(kv[0]), dev.tensor(kv[1]))
+        got = c.attention(dev.tensor(q), 0, 0.125).numpy()
+        first = max(32, 33 if n < 64 else 32) - past   # (a bad row past the last whole block is one row)
+        assert np.isfinite(got[:first]).all() and np.isnan(got[first:]).all()
+        check(got[:first], q[:first], kv[0][:32], kv[1][:32], 0.125, "before") if first == 32 - past else None
+
+
+@pytest.mark.parametrize("S,past,H", [(1, 0, 4), (1, 190, 4), (60, 140, 4), (100, 140, 256), (140, 100, 256)])
+@pytest.mark.parametrize("power", [20, 27, 40])
+def test_values_of_blocks_far_apart(dev, S, past, H, power):
+    """Blocks of V whose sizes lie up to 2^40 apart (zeros among them), seen with weights alike: each
+    weight counts with its full precision in the sum, and the large values with theirs in the result."""
+    n = S + past
+    k, v = rows(12, n, 2, 64)
+    size = np.array([8, 8 - power, 8 - power, 8 - power, None, 8 - power // 2, -14], dtype=object)
+    for b in range((n + 31) // 32):
+        e = size[b % 7]
+        blk = v[32 * b:32 * b + 32].astype(np.float64)
+        blk = blk / np.abs(blk).max(axis=(0, 2), keepdims=True)
+        v[32 * b:32 * b + 32] = 0 if e is None else np.maximum(np.abs(blk) * 2.0 ** max(e, -24), 2.0 ** -24) * np.sign(blk)
+    q = (np.random.default_rng(n).standard_normal((S, H, 64)) / 4).astype(np.float16)
+    c = KVCache(dev, 1, n, 2, 64, Q8_0)
+    c.set(0, dev.tensor(k), dev.tensor(v))
+    got = c.attention(dev.tensor(q), 0, 0.125).numpy()
+    kk, vv = held(k), held(v)
+    ref, tol = attend(q, kk, vv, 0.125)
+    for h in range(H):
+        sc = np.where(np.arange(n)[None, :] <= np.arange(S)[:, None] + past, (q[:, h].astype(np.float64) @ kk[:, h // (H // 2)].T) * 0.125, -np.inf)
+        p = np.exp(sc - sc.max(1, keepdims=True))
+        assert p[p > 0].min() > 2.0 ** -12   # all weights are of normal size: attend()'s term for the smaller ones falls away
+        p /= p.sum(1, keepdims=True)
+        absum = p @ np.abs(vv[:, h // (H // 2)])
+        dsc = 70 * 2.0 ** -24 * (np.abs(q[:, h].astype(np.float64)) @ np.abs(kk[:, h // (H // 2)]).T) * 0.125 + 2.0 ** -22 * (np.abs(np.where(sc > -np.inf, sc, 0)) + 40)
+        t = 2.0 ** -11 * (np.abs(ref[:, h]) + 2 * absum) + (2 * dsc.max(1, keepdims=True) + n * 2.0 ** -24) * absum + 2.0 ** -25
+        assert (np.abs(got[:, h] - ref[:, h]) <= t).all(), float((np.abs(got[:, h] - ref[:, h]) / t).max())
+
+
 def test_an_infinite_query_spoils_its_row_only(dev):
     k, v = rows(7, 60, 2, 64)
     q = np.random.default_rng(7).standard_normal((20, 4, 64)).astype(np.float16)
