@@ -98,7 +98,9 @@ __device__ __forceinline__ float at(const LogprobArgs& a, size_t i) {
     return F32 ? ((const float*)a.x)[i] : h2f(((const uint16_t*)a.x)[i]);
 }
 
-// 32 elements of a thread, in vectors of 16 bytes a workgroup's width apart.
+// 32 elements of a thread, in vectors of 16 bytes a workgroup's width apart, of
+// a batch that ends at element hi: the vectors past it are moved back to end
+// there, and what they repeat counts for none.
 struct __attribute__((packed, aligned(4))) f4_any {
     float f[4];
 };
@@ -107,17 +109,35 @@ struct Batch {
     static constexpr int W = F32 ? 4 : 8, NV = 32 / W;
     float f[F32 ? 32 : 1];
     h8 h[F32 ? 1 : 4];
-    static __device__ __forceinline__ int index(int j) { return (j / W * 256 + (int)threadIdx.x) * W + j % W; }
+    int lo, hi, last;   // elements lo .. hi - 1 are new; the last vector's place
     __device__ __forceinline__ float operator[](int j) const {
         if constexpr (F32) return f[j];
         else return (float)h[j / 8][j % 8];
     }
-    // Elements base + index(j), a batch of the row.  (No branch among the
-    // loads: each would wait for those before it.)
-    __device__ __forceinline__ void load(const LogprobArgs& a, size_t base) {
+    static __device__ __forceinline__ int place(int v) { return (v * 256 + (int)threadIdx.x) * W; }
+    __device__ __forceinline__ int index(int j) const { return min(place(j / W), last) + j % W; }
+    __device__ __forceinline__ bool mine(int j) const {
+        const int i = index(j);
+        return i >= lo && i >= place(j / W) && i < hi;
+    }
+    __device__ __forceinline__ void set(int j, float x) {
+        if constexpr (F32) f[j] = x;
+        else h[j / 8][j % 8] = (h16)x;
+    }
+    // Elements base + index(j); -inf in place of those that are not new.  (No
+    // branch among the loads: each would wait for those before it.)
+    __device__ __forceinline__ void load(const LogprobArgs& a, size_t base, int lo_, int hi_) {
+        lo = lo_;
+        hi = hi_;
+        last = hi > W ? hi - W : 0;
+        if (hi < W) {   // a row shorter than a vector
+#pragma unroll
+            for (int j = 0; j < 32; j++) set(j, j < W && threadIdx.x == 0 && j < hi ? at<F32>(a, base + j) : -INFINITY);
+            return;
+        }
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const size_t i = base + (v * 256 + (int)threadIdx.x) * W;
+            const size_t i = base + min(place(v), last);
             if constexpr (F32) {
                 const f4_any w = *(const f4_any*)((const float*)a.x + i);
 #pragma unroll
@@ -127,32 +147,10 @@ struct Batch {
                 h[v] = __builtin_bit_cast(h8, u4{w.w[0], w.w[1], w.w[2], w.w[3]});
             }
         }
-    }
-    // The same of a row of `have` elements, less than a batch; -inf past them.
-    __device__ __forceinline__ void load_short(const LogprobArgs& a, size_t base, int have) {
+        if (lo || hi < kBatch)
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            const int i = (v * 256 + (int)threadIdx.x) * W;
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                if constexpr (F32) f[4 * v + e] = -INFINITY;
-                else h[v][e] = (h16)-INFINITY;
-            }
-            if (i >= have) continue;
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                if constexpr (F32) f[4 * v + e] = i + e < have ? ((const float*)a.x)[base + i + e] : -INFINITY;
-                else h[v][e] = i + e < have ? __builtin_bit_cast(h16, ((const uint16_t*)a.x)[base + i + e]) : (h16)-INFINITY;
-            }
-        }
-    }
-    // -inf in place of the elements before index lo
-    __device__ __forceinline__ void drop_before(int lo) {
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-            if constexpr (F32) f[j] = index(j) < lo ? -INFINITY : f[j];
-            else h[j / 8][j % 8] = index(j) < lo ? (h16)-INFINITY : h[j / 8][j % 8];
-        }
+            for (int j = 0; j < 32; j++)
+                if (!mine(j)) set(j, -INFINITY);
     }
 };
 
@@ -267,13 +265,10 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         if (tid == 0) sh.count = sh.kept = 0;
     }
     for (int b = 0, nb = 0; b < count; b += kBatch, nb++) {
-        // The last batch of several is moved back to be whole: its elements
-        // from lo on are new.  A row shorter than a batch ends at hi.
-        const int at0 = count - b < kBatch && nb ? count - kBatch : b, lo = b - at0, hi = count - at0;
+        // the last batch of several is moved back to be whole
+        const int at0 = count - b < kBatch && nb ? count - kBatch : b;
         Batch<F32> x;
-        if (hi >= kBatch) x.load(a, base + at0);
-        else x.load_short(a, base, hi);
-        if (lo) x.drop_before(lo);
+        x.load(a, base + at0, b - at0, count - at0 < kBatch ? count - at0 : kBatch);
         float m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 32; j++) m = fmaxf(m, x[j]);
@@ -281,17 +276,16 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int j = 0; j < 32; j++) s.add(x[j]);
         if constexpr (TOP) {
-            auto mine = [&](int j) { return Batch<F32>::index(j) >= lo && Batch<F32>::index(j) < hi; };
-            if ((!best || m > key_value(best)) && (mine(0) || mine(31))) {
+            if (!best || m > key_value(best)) {
                 // the first element that is m (an -inf in place of another is none)
                 int first = -1;
                 if (m > -INFINITY) {
 #pragma unroll
                     for (int j = 31; j >= 0; j--) first = x[j] == m ? j : first;
                 } else {
-                    for (int j = 31; j >= 0; j--) first = x[j] == m && mine(j) ? j : first;
+                    for (int j = 31; j >= 0; j--) first = x[j] == m && x.mine(j) ? j : first;
                 }
-                if (first >= 0) best = key_of(m, begin + at0 + Batch<F32>::index(first));
+                if (first >= 0) best = key_of(m, begin + at0 + x.index(first));
             }
             if (nb == 0) tau = bound(best, a.n_top, sh);
             const float least = tau ? key_value(tau) : -INFINITY;
@@ -305,13 +299,13 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
                 }
                 const int last = tau ? key_index(tau) - begin - at0 : kBatch;
                 for (; even; even &= even - 1) {
-                    const int j = __builtin_ctz(even), i = Batch<F32>::index(j);
-                    if (i >= lo && i < hi && i <= last) hit |= 1u << j;
+                    const int j = __builtin_ctz(even);
+                    if (x.mine(j) && x.index(j) <= last) hit |= 1u << j;
                 }
                 if (hit) {
                     int slot = atomicAdd(&sh.count, __builtin_popcount(hit));
                     for (; hit; hit &= hit - 1, slot++)
-                        if (slot < kList) sh.list[slot] = at0 + Batch<F32>::index(__builtin_ctz(hit));
+                        if (slot < kList) sh.list[slot] = at0 + x.index(__builtin_ctz(hit));
                 }
             }
             if (nb && !(nb & (nb + 1)) && b + kBatch < count) tau = bound(best, a.n_top, sh);
