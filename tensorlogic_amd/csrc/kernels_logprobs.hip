@@ -28,7 +28,11 @@ namespace tlhip {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
-constexpr int kBatch = 8192;      // elements of a workgroup's batch: 32 per thread
+// Elements of a thread's batch, for rows that need more than 256 * kShort
+// threads' and for the others (2000 f16 rows of 501, 5 alternatives: 11.4 us
+// against 22 with the long batch).
+constexpr int kLong = 32, kShort = 8;
+constexpr int kBatch = 256 * kLong;     // elements of a workgroup's
 constexpr int kList = 2048, kRanked = 512;
 constexpr int kMaxChunks = 32;
 
@@ -98,17 +102,17 @@ __device__ __forceinline__ float at(const LogprobArgs& a, size_t i) {
     return F32 ? ((const float*)a.x)[i] : h2f(((const uint16_t*)a.x)[i]);
 }
 
-// 32 elements of a thread, in vectors of 16 bytes a workgroup's width apart, of
+// E elements of a thread, in vectors of 16 bytes a workgroup's width apart, of
 // a batch that ends at element hi: the vectors past it are moved back to end
 // there, and what they repeat counts for none.
 struct __attribute__((packed, aligned(4))) f4_any {
     float f[4];
 };
-template <bool F32>
+template <bool F32, int E>
 struct Batch {
-    static constexpr int W = F32 ? 4 : 8, NV = 32 / W;
-    float f[F32 ? 32 : 1];
-    h8 h[F32 ? 1 : 4];
+    static constexpr int W = F32 ? 4 : 8, NV = E / W, SIZE = 256 * E;
+    float f[F32 ? E : 1];
+    h8 h[F32 ? 1 : NV];
     int lo, hi, last;   // elements lo .. hi - 1 are new; the last vector's place
     __device__ __forceinline__ float operator[](int j) const {
         if constexpr (F32) return f[j];
@@ -132,7 +136,7 @@ struct Batch {
         last = hi > W ? hi - W : 0;
         if (hi < W) {   // a row shorter than a vector
 #pragma unroll
-            for (int j = 0; j < 32; j++) set(j, j < W && threadIdx.x == 0 && j < hi ? at<F32>(a, base + j) : -INFINITY);
+            for (int j = 0; j < E; j++) set(j, j < W && threadIdx.x == 0 && j < hi ? at<F32>(a, base + j) : -INFINITY);
             return;
         }
 #pragma unroll
@@ -147,9 +151,9 @@ struct Batch {
                 h[v] = __builtin_bit_cast(h8, u4{w.w[0], w.w[1], w.w[2], w.w[3]});
             }
         }
-        if (lo || hi < kBatch)
+        if (lo || hi < SIZE)
 #pragma unroll
-            for (int j = 0; j < 32; j++)
+            for (int j = 0; j < E; j++)
                 if (!mine(j)) set(j, -INFINITY);
     }
 };
@@ -249,7 +253,7 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Stat
     }
 }
 
-template <bool F32, bool TOP>
+template <bool F32, bool TOP, int E>
 __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     __shared__ Stat<F32> st[4];
     __shared__ __align__(16) uint8_t top_raw[TOP ? sizeof(TopShared) : 16];
@@ -264,26 +268,26 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         if (tid < kMaxTop) top[tid] = 0;
         if (tid == 0) sh.count = sh.kept = 0;
     }
-    for (int b = 0, nb = 0; b < count; b += kBatch, nb++) {
+    for (int b = 0, nb = 0; b < count; b += Batch<F32, E>::SIZE, nb++) {
         // the last batch of several is moved back to be whole
-        const int at0 = count - b < kBatch && nb ? count - kBatch : b;
-        Batch<F32> x;
-        x.load(a, base + at0, b - at0, count - at0 < kBatch ? count - at0 : kBatch);
+        const int at0 = count - b < Batch<F32, E>::SIZE && nb ? count - Batch<F32, E>::SIZE : b;
+        Batch<F32, E> x;
+        x.load(a, base + at0, b - at0, count - at0 < Batch<F32, E>::SIZE ? count - at0 : Batch<F32, E>::SIZE);
         float m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 32; j++) m = fmaxf(m, x[j]);
+        for (int j = 0; j < E; j++) m = fmaxf(m, x[j]);
         if (m > s.m) s.rise(m);
 #pragma unroll
-        for (int j = 0; j < 32; j++) s.add(x[j]);
+        for (int j = 0; j < E; j++) s.add(x[j]);
         if constexpr (TOP) {
             if (!best || m > key_value(best)) {
                 // the first element that is m (an -inf in place of another is none)
                 int first = -1;
                 if (m > -INFINITY) {
 #pragma unroll
-                    for (int j = 31; j >= 0; j--) first = x[j] == m ? j : first;
+                    for (int j = E - 1; j >= 0; j--) first = x[j] == m ? j : first;
                 } else {
-                    for (int j = 31; j >= 0; j--) first = x[j] == m && x.mine(j) ? j : first;
+                    for (int j = E - 1; j >= 0; j--) first = x[j] == m && x.mine(j) ? j : first;
                 }
                 if (first >= 0) best = key_of(m, begin + at0 + x.index(first));
             }
@@ -293,11 +297,11 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
                 // the places of the batch's keys from tau up go to the list
                 uint32_t hit = 0, even = 0;
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
+                for (int j = 0; j < E; j++) {
                     hit |= x[j] > least ? 1u << j : 0;
                     even |= x[j] == least ? 1u << j : 0;
                 }
-                const int last = tau ? key_index(tau) - begin - at0 : kBatch;
+                const int last = tau ? key_index(tau) - begin - at0 : Batch<F32, E>::SIZE;
                 for (; even; even &= even - 1) {
                     const int j = __builtin_ctz(even);
                     if (x.mine(j) && x.index(j) <= last) hit |= 1u << j;
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
                         if (slot < kList) sh.list[slot] = at0 + x.index(__builtin_ctz(hit));
                 }
             }
-            if (nb && !(nb & (nb + 1)) && b + kBatch < count) tau = bound(best, a.n_top, sh);
+            if (nb && !(nb & (nb + 1)) && b + Batch<F32, E>::SIZE < count) tau = bound(best, a.n_top, sh);
         }
     }
     for (int k = 32; k; k >>= 1) s.join(s.from_lane(k));
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     s = st[0];
     for (int k = 1; k < 4; k++) s.join(st[k]);
     if constexpr (TOP) {
-        if (count > kBatch) tau = bound(best, a.n_top, sh);   // (else it stands)
+        if (count > Batch<F32, E>::SIZE) tau = bound(best, a.n_top, sh);   // (else it stands)
         const int listed = sh.count;
         auto listed_key = [&](int i) { return key_of(at<F32>(a, base + sh.list[i]), begin + sh.list[i]); };
         if (listed <= kList) {
@@ -371,7 +375,9 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
 }  // namespace
 
 // Chunks of a row: enough workgroups for two to a CU, and no more than one for
-// each batch of a row.
+// each batch of a row.  (333 f32 rows of 51200 with 20 alternatives: 26.3 us,
+// with one to a CU 27.2, three 28.8, four 30.9; 700 f16 rows of 128000, 5:
+// 56.5, from three on 64.)
 constexpr int kWorkgroups = 512;
 LogprobPlan logprobs_plan(int rows, int V, int n_top) {
     LogprobPlan p;
@@ -389,17 +395,17 @@ LogprobPlan logprobs_plan(int rows, int V, int n_top) {
     return p;
 }
 
-tlhip_status launch_logprobs(hipStream_t s, const LogprobArgs& a) {
+template <bool F32, int E>
+void launch(hipStream_t s, const LogprobArgs& a) {
     const unsigned wg = (unsigned)a.rows * a.chunks;
-    if (a.f32) {
-        if (a.n_top) logprobs_kernel<true, true><<<wg, 256, 0, s>>>(a);
-        else logprobs_kernel<true, false><<<wg, 256, 0, s>>>(a);
-        if (a.chunks > 1) logprobs_join_kernel<true><<<a.rows, 256, 0, s>>>(a);
-    } else {
-        if (a.n_top) logprobs_kernel<false, true><<<wg, 256, 0, s>>>(a);
-        else logprobs_kernel<false, false><<<wg, 256, 0, s>>>(a);
-        if (a.chunks > 1) logprobs_join_kernel<false><<<a.rows, 256, 0, s>>>(a);
-    }
+    if (a.n_top) logprobs_kernel<F32, true, E><<<wg, 256, 0, s>>>(a);
+    else logprobs_kernel<F32, false, E><<<wg, 256, 0, s>>>(a);
+    if (a.chunks > 1) logprobs_join_kernel<F32><<<a.rows, 256, 0, s>>>(a);
+}
+
+tlhip_status launch_logprobs(hipStream_t s, const LogprobArgs& a) {
+    if (a.V <= 256 * kShort) a.f32 ? launch<true, kShort>(s, a) : launch<false, kShort>(s, a);
+    else a.f32 ? launch<true, kLong>(s, a) : launch<false, kLong>(s, a);
     return TLHIP_OK;
 }
 
