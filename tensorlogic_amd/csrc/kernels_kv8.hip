@@ -10,7 +10,7 @@
 // calls brought them, and no value is rounded twice.
 //
 // A block or tail of one head is a tile in the order in which the attention
-// kernel's lanes read it (Kv8Tile), so that every load is 16 bytes per lane
+// kernel's lanes read it, so that every load is 16 bytes per lane
 // and contiguous over the wave, and neither keys nor probabilities are
 // shuffled between lanes:
 //   K tile  [D/8][32 keys][8]: 8 dims of a key together
@@ -234,6 +234,11 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read p) {
 // loses bits to f16's range only below 2^-13 of the row's largest.  Scores,
 // weights, sums and O are f32; P's rounding to f16 (2^-11 relative, for the
 // matrix cores) is the only one before the result's.
+//
+// Bound: a step of one row by reading K and V (65000 keys of 32 heads of 80,
+// 333 MB, 62 us: 5.3 TB/s); prompts by the vector work of a score and of the
+// unpacking (2048 rows of 32 / 4 heads of 64 37.6 us, 457 TFLOP/s; 700 after
+// 5300 of 32 / 8 of 128 93 us, 700 TFLOP/s).
 constexpr float kLog2e = 1.44269504088896f;
 constexpr float kNone = -3.0e38f;   // M before any key
 
@@ -670,16 +675,26 @@ tlhip_status launch_kv8_read(hipStream_t s, const Kv8Read& p) {
     return TLHIP_OK;
 }
 
-// How a call is spread over the device: rows of many queries take a wave each
-// (splits = 0); few rows split their keys.
+// How a call is spread over the device.  A wave takes two columns of 16 rows
+// when there are more rows than one has (a tile is unpacked once for both:
+// 2048 rows of 32 / 4 heads of 64 37.6 us against 48 with one and 65 with
+// four; 700 after 5300 93 against 167), one at head dim 256, whose sums fill
+// the registers.  With 2048 or more such columns a wave walks all keys of its
+// own (splits = 0: 2048 rows of 32 / 8 heads of 128 61 us against 72), with
+// fewer the four waves of a workgroup share the keys (1024 rows of 32 heads of
+// 80: 21 us against 28); and below 512 workgroups the keys are cut into
+// splits, up to two workgroups a CU, four tiles each at least.  (Up to four a
+// CU: 300 rows after 3000, 32 / 4 heads of 64, 35 us against 25, one row after
+// 20000, 32 / 8 of 128, 17.4 against 13.9; up to one: 12.2 there, but 65000
+// keys of 32 heads of 80 67.7 against 64.5.)
 Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     Kv8Plan pl;
     const int64_t rows = (int64_t)S * group;
     const int tiles = (len + 31) / 32;
     pl.nq = rows <= 16 || D > 128 ? 1 : 2;
     const int64_t wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * n_kv;
-    if (wg >= 1024) return pl;
-    int64_t splits = 1024 / wg;
+    if (wg >= 2048) return pl;
+    int64_t splits = 512 / wg;
     if (splits < 1) splits = 1;
     if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
     pl.splits = (int)splits;

@@ -139,7 +139,9 @@ def test_attention(dev, H, kv, D, S, past):
 
 
 @pytest.mark.parametrize("H,kv,D,S,past", [(32, 4, 64, 300, 0), (32, 32, 80, 40, 100), (16, 1, 64, 1, 5000), (8, 8, 128, 1, 4111),
-                                           (40, 1, 64, 1, 500), (128, 2, 32, 3, 100), (4, 1, 64, 700, 1300), (64, 64, 64, 17, 333)])
+                                           (40, 1, 64, 1, 500), (128, 2, 32, 3, 100), (4, 1, 64, 700, 1300), (64, 64, 64, 17, 333),
+                                           # enough rows for a wave to take all keys of its own
+                                           (256, 8, 32, 260, 37), (256, 8, 64, 260, 300), (512, 4, 80, 135, 1), (256, 16, 128, 260, 0), (256, 1, 256, 131, 20)])
 def test_attention_larger(dev, H, kv, D, S, past):
     test_attention(dev, H, kv, D, S, past)
 
@@ -205,7 +207,7 @@ def test_rows_before_a_bad_block_in_one_tile_of_rows(dev, S, past):
         check(got[:first], q[:first], kv[0][:32], kv[1][:32], 0.125, "before") if first == 32 - past else None
 
 
-@pytest.mark.parametrize("S,past,H", [(1, 0, 4), (1, 190, 4), (60, 140, 4), (100, 140, 256), (140, 100, 256)])
+@pytest.mark.parametrize("S,past,H", [(1, 0, 4), (1, 190, 4), (60, 140, 4), (100, 140, 256), (140, 100, 512)])
 @pytest.mark.parametrize("power", [20, 27, 40])
 def test_values_of_blocks_far_apart(dev, S, past, H, power):
     """Blocks of V whose sizes lie up to 2^40 apart (zeros among them), seen with weights alike: each
