@@ -18,6 +18,11 @@
 // great length) overflow the list and are ranked by n rounds over the row.
 //
 // Few rows are cut into chunks, a workgroup each, joined by a second kernel.
+//
+// Bound by memory without alternatives (2048 f16 rows of 32000: 28.6 us, 4.6
+// TB/s), with them by the exps and the list beside the loads (333 f32 rows of
+// 51200, 20 alternatives: 21 us and 4 for the join, 2.7 TB/s), for one row by
+// the two launches (32000 f16: 7 and 3 us).
 #include <cmath>
 
 #include "device_common.hpp"

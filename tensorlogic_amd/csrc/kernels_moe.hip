@@ -8,6 +8,10 @@
 // Weights are the f16 values that their packed types stand for, as in
 // linear(); everything between x and y is f32, rounded once.
 //
+// One token of 8 Q4_0 experts 2048 x 5632, two chosen: 20.5 us a call (router
+// 3.6, gate and up 8 to 10, down 7 to 8); 13 tokens, Q8_0: 74 us (gate and up
+// 41, 4.7 TB/s; down 26; router and sum 4 each).
+//
 // Four launches: the router (a workgroup per token); gate and up; down; the
 // sum over a token's experts (three for one token, whose down sums them
 // itself).  What bounds the middle two is reading the weights of the experts
