@@ -284,7 +284,10 @@ tlhip_status tlhip_temperature_sample(tlhip_ctx ctx, tlhip_tensor logits, float 
  * entropy and top_logprob are F32.  -inf logits have probability 0 and their
  * log probability is -inf.  A row with a NaN or +inf, or of -inf alone, has
  * no distribution: NaN, and top_ids -1.  An id outside [0, V) gives NaN.
- * n_top <= min(64, V), V <= 2^30, fewer than 2^24 rows.                    */
+ * n_top <= min(64, V), V <= 2^30, fewer than 2^24 rows.  Tensors of another
+ * context of the device may take part (here, in tlhip_moe and with an 8-bit
+ * cache): the call comes after what is queued there, and before what is
+ * queued there later.                                                      */
 tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tensor ids, int n_top,
                                   tlhip_tensor logprob, tlhip_tensor entropy, tlhip_tensor top_logprob,
                                   tlhip_tensor top_ids);

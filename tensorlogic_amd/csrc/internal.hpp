@@ -16,6 +16,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <unordered_map>
@@ -141,6 +142,16 @@ tlhip_status check_dtype(tlhip_tensor t, tlhip_dtype d, const char* op);
 tlhip_status after_launch(tlhip_ctx ctx, const char* op);
 // A tensor of ctx's device (another device's is refused).
 tlhip_status check_here(tlhip_ctx ctx, tlhip_tensor t, const char* op);
+// Tensors of a call that another context of the device made: the call's work
+// comes after what is queued on their streams (wait) and before what is queued
+// there later (done).
+struct OtherStreams {
+    tlhip_ctx ctx, other[8];
+    int n = 0;
+    explicit OtherStreams(tlhip_ctx c) : ctx(c) {}
+    tlhip_status wait(std::initializer_list<tlhip_tensor> tensors);   // null tensors do not count
+    tlhip_status done();
+};
 // Makes a device current for a call and puts the caller's back.
 struct DeviceScope {
     int prev = -1;

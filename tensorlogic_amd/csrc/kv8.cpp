@@ -57,6 +57,8 @@ tlhip_status kv8_write(tlhip_ctx ctx, tlhip_kvcache c, int layer, tlhip_tensor k
     TLHIP_TRY(check_here(ctx, k, "kvcache K"));
     TLHIP_TRY(check_here(ctx, v, "kvcache V"));
     DeviceScope scope(ctx->device);
+    OtherStreams others(ctx);
+    TLHIP_TRY(others.wait({k, v}));
     Kv8Layer& l = c->q8[layer];
     Kv8Write p;
     p.k = (const uint16_t*)k->data;
@@ -80,6 +82,7 @@ tlhip_status kv8_write(tlhip_ctx ctx, tlhip_kvcache c, int layer, tlhip_tensor k
     p.n_blocks = n_blocks(c);
     TLHIP_TRY(launch_kv8_write(ctx->stream, p));
     TLHIP_TRY(after_launch(ctx, "kvcache write"));
+    TLHIP_TRY(others.done());
     l.tail_cur = p.tail_dst;
     return TLHIP_OK;
 }
@@ -130,6 +133,8 @@ tlhip_status kv8_attention(tlhip_ctx ctx, tlhip_tensor q, tlhip_kvcache c, int l
         return fail(TLHIP_ERR_SHAPE_MISMATCH, "attention q/out: shape %s vs %s", shape_str(q).c_str(), shape_str(out).c_str());
     if (S * H > INT32_MAX / 4) return fail(TLHIP_ERR_INVALID_DIMENSION, "attention: q %s is too large", shape_str(q).c_str());
     DeviceScope scope(ctx->device);
+    OtherStreams others(ctx);
+    TLHIP_TRY(others.wait({q, out}));
     const Kv8Layer& l = c->q8[layer];
     const int len = c->len[layer];
     Kv8Attn p;
@@ -158,7 +163,8 @@ tlhip_status kv8_attention(tlhip_ctx ctx, tlhip_tensor q, tlhip_kvcache c, int l
         if (!p.scratch) return fail(TLHIP_ERR_ALLOCATION, "attention: no workspace of %zu bytes", pl.scratch_bytes);
     }
     TLHIP_TRY(launch_kv8_attention(ctx->stream, p, pl));
-    return after_launch(ctx, "attention");
+    TLHIP_TRY(after_launch(ctx, "attention"));
+    return others.done();
 }
 
 }  // namespace tlhip

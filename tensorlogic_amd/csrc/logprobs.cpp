@@ -53,6 +53,8 @@ extern "C" tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits,
     a.n_top = n_top;
     a.f32 = logits->dtype == TLHIP_F32;
     DeviceScope scope(ctx->device);
+    OtherStreams others(ctx);
+    TLHIP_TRY(others.wait({logits, ids, logprob, entropy, top_logprob, top_ids}));
     const LogprobPlan pl = logprobs_plan(a.rows, a.V, n_top);
     a.chunks = pl.chunks;
     a.chunk = pl.chunk;
@@ -63,5 +65,6 @@ extern "C" tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits,
         a.part_keys = (uint64_t*)(ws + pl.part_bytes);
     }
     TLHIP_TRY(launch_logprobs(ctx->stream, a));
-    return after_launch(ctx, op);
+    TLHIP_TRY(after_launch(ctx, op));
+    return others.done();
 } TLHIP_CATCH_STATUS

@@ -61,6 +61,8 @@ extern "C" tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor ro
     const size_t at_max = at_h + align256(pairs * I * sizeof(float)), at_part = at_max + align256(pairs * (I / 16) * sizeof(float));
     const size_t need = at_part + pairs * K * sizeof(float);
     DeviceScope scope(ctx->device);
+    OtherStreams others(ctx);
+    TLHIP_TRY(others.wait({x, router, gate, up, down, y}));
     uint8_t* ws = (uint8_t*)ctx_workspace(ctx, need);
     if (!ws) return fail(TLHIP_ERR_ALLOCATION, "moe: no workspace of %zu bytes", need);
     MoeArgs a;
@@ -89,5 +91,6 @@ extern "C" tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor ro
         a.M = (int)(M - m < kSlab ? M - m : kSlab);
         TLHIP_TRY(launch_moe(ctx->stream, a));
     }
-    return after_launch(ctx, "moe");
+    TLHIP_TRY(after_launch(ctx, "moe"));
+    return others.done();
 } TLHIP_CATCH_STATUS

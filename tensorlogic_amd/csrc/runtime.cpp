@@ -138,6 +138,35 @@ tlhip_status check_here(tlhip_ctx ctx, tlhip_tensor t, const char* op) {
     return TLHIP_OK;
 }
 
+// What is queued on `later` from here on waits for what `first` has now.
+static tlhip_status order_streams(hipStream_t first, hipStream_t later) {
+    hipEvent_t ev = nullptr;
+    TLHIP_CHECK_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+    hipError_t e = hipEventRecord(ev, first);
+    if (e == hipSuccess) e = hipStreamWaitEvent(later, ev, 0);
+    (void)hipEventDestroy(ev);   // (released once it has been reached)
+    TLHIP_CHECK_HIP(e);
+    return TLHIP_OK;
+}
+
+tlhip_status OtherStreams::wait(std::initializer_list<tlhip_tensor> tensors) {
+    for (tlhip_tensor t : tensors) {
+        if (!t || t->ctx == ctx) continue;
+        bool known = false;
+        for (int i = 0; i < n; i++) known |= other[i] == t->ctx;
+        if (known) continue;
+        if (n == 8) return fail(TLHIP_ERR_INVALID_ARGUMENT, "tensors of more than 8 other contexts");
+        TLHIP_TRY(order_streams(t->ctx->stream, ctx->stream));
+        other[n++] = t->ctx;
+    }
+    return TLHIP_OK;
+}
+
+tlhip_status OtherStreams::done() {
+    for (int i = 0; i < n; i++) TLHIP_TRY(order_streams(ctx->stream, other[i]->stream));
+    return TLHIP_OK;
+}
+
 tlhip_status after_launch(tlhip_ctx ctx, const char* op) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(TLHIP_ERR_DEVICE, "%s launch failed: %s", op, hipGetErrorString(e));

@@ -98,6 +98,15 @@ def test_larger(dev, M, E, K, I, top, gu):
     run(dev, 2, M, E, K, I, top, True, gu, gu)
 
 
+@pytest.mark.parametrize("t", [F16, Q4_0, Q8_0])
+@pytest.mark.parametrize("M", [1, 2, 9, 16, 17, 40])
+@pytest.mark.parametrize("K,I", [(16384, 32), (32, 16384), (16384, 64), (96, 16352)])
+def test_longest_rows(dev, t, M, K, I):
+    """What a workgroup keeps in LDS is largest here.  (All experts where K is long: the bound of a sum
+    of 16384 products leaves doubt about which two of three are chosen.)"""
+    run(dev, 4, M, 3, K, I, 3 if K == 16384 else 2, False, t, t)
+
+
 def test_all_tokens_choose_one_expert_and_the_same_row_twice(dev):
     r = np.random.default_rng(5)
     x = np.repeat(r.standard_normal((1, 128)), 40, 0).astype(np.float16)

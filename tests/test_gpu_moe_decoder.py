@@ -5,7 +5,8 @@ against 64-bit arithmetic on the values that it was given."""
 import numpy as np
 import pytest
 
-from tensorlogic_amd import F16, I32, Q4_0, Q8_0, KVCache, embedding, moe, token_logprobs
+from tensorlogic_amd import F16, F32, I32, Q4_0, Q8_0, Device, KVCache, embedding, moe, token_logprobs
+from tensorlogic_amd._lib import call
 from test_gpu_kv8 import as_f16, check, held
 from test_gpu_logprobs import close
 from test_gpu_logprobs import reference as logprobs_reference
@@ -76,3 +77,51 @@ def test_prompt_and_tokens(dev, H, kv, D, gu, dn):
         again.append(b.step(ids[past:past + s], past)[0])
         past += s
     assert np.array_equal(again[-1][6], logits) and all(np.array_equal(x, z) for x, z in zip(again[-1][7:], said))
+
+
+def test_tensors_of_another_context(dev):
+    """Inputs still being computed on another context's stream, results read and inputs overwritten on it."""
+    r = np.random.default_rng(3)
+    M, E, K, I, top, V = 12, 4, 256, 96, 2, 3001
+    w = dev.tensor((r.standard_normal((K, K)) / 16).astype(np.float16))
+    wide = dev.tensor((r.standard_normal((4096, K)) / 16).astype(np.float16))
+    back = dev.tensor((r.standard_normal((K, 4096)) / 64).astype(np.float16))
+    x0 = dev.tensor(r.standard_normal((M, K)).astype(np.float16))
+    router, mats = case(6, E, K, I, F16, F16)
+    experts = [dev.tensor(m[0]) for m in mats]
+    head = dev.tensor((r.standard_normal((V, K)) / 16).astype(np.float16))
+    ids = r.integers(0, V, M).astype(np.int32)
+
+    def chain():   # some hundred launches
+        x = x0
+        for _ in range(60):
+            x = x.linear(w).linear(wide).linear(back)
+            x = x.rms_norm([K], dev.tensor(np.ones(K, np.float16)))
+        return x
+
+    x = chain()
+    keys = x.linear(w).reshape((M, 4, 64))
+    c = KVCache(dev, 1, 64, 4, 64, Q8_0)
+    c.set(0, keys, keys)
+    want = [moe(x, dev.tensor(router), *experts, top).numpy(), c.attention(keys, 0, 0.125).numpy(),
+            *(t.numpy() for t in token_logprobs(x.linear(head), dev.tensor(ids, I32), 3))]
+    other = Device(0)
+    try:
+        o_router, o_ids = other.tensor(router), other.tensor(ids, I32)
+        y, att = other.empty((M, K)), other.empty((M, 4, 64))
+        lp, h, tl, ti = other.empty((M,), F32), other.empty((M,), F32), other.empty((M, 3), F32), other.empty((M, 3), I32)
+        oc = KVCache(other, 1, 64, 4, 64, Q8_0)
+        x = chain()
+        keys = x.linear(w).reshape((M, 4, 64))
+        logits = x.linear(head)
+        call("tlhip_kvcache_set", other.h, oc.h, 0, keys.h, keys.h)
+        call("tlhip_attention_prefill", other.h, keys.h, oc.h, 0, 0.125, att.h)
+        call("tlhip_moe", other.h, x.h, o_router.h, *(e.h for e in experts), top, 1, y.h)
+        call("tlhip_token_logprobs", other.h, logits.h, o_ids.h, 3, lp.h, h.h, tl.h, ti.h)
+        del x, keys, logits   # their blocks go to dev's next tensors
+        junk = [dev.tensor(np.full((M, n), 7.0, np.float16)).mul_scalar(3.0) for n in (K, K, V, V)]
+        got = [t.numpy() for t in (y, att, lp, h, tl, ti)]
+        assert all(np.array_equal(a, b) for a, b in zip(want, got))
+        del junk, o_router, o_ids, y, att, lp, h, tl, ti, oc
+    finally:
+        other.close()
