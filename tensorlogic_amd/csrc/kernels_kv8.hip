@@ -237,8 +237,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read p) {
 //
 // Bound: a step of one row by reading K and V (65000 keys of 32 heads of 80,
 // 333 MB, 62 us: 5.3 TB/s); prompts by the vector work of a score and of the
-// unpacking (2048 rows of 32 / 4 heads of 64 37.6 us, 457 TFLOP/s; 700 after
-// 5300 of 32 / 8 of 128 93 us, 700 TFLOP/s).
+// unpacking (2048 rows of 32 / 4 heads of 64 31.3 us, 550 TFLOP/s; 700 after
+// 5300 of 32 / 8 of 128 91.5 us, 708 TFLOP/s).
 constexpr float kLog2e = 1.44269504088896f;
 constexpr float kNone = -3.0e38f;   // M before any key
 
@@ -502,9 +502,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_rows_kernel(Kv
     w.store(p, head, row0, rows);
 }
 
-// Few rows: the keys of NQ * 16 rows split over gridDim's splits and a
-// workgroup's four waves, which join through LDS; the splits' sums go to
-// scratch for kv8_join_kernel.
+// The keys of NQ * 16 rows shared by a workgroup's four waves, which join
+// through LDS, and with few rows by gridDim's splits, whose sums go to scratch
+// for kv8_join_kernel.  Later rows see more keys: they start first.
 template <int D, int NQ>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_keys_kernel(Kv8Attn p) {
     constexpr int NC = (D + 31) / 32;
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_keys_kernel(Kv
     __shared__ float sm[4][16 * NQ], sl[4][16 * NQ];
     const int rows = p.S * p.group;
     const int split = blockIdx.x % p.splits, head = blockIdx.x / p.splits % p.n_kv;
-    const int row0 = (int)(blockIdx.x / p.splits / p.n_kv) * (16 * NQ);
+    const int row0 = ((rows - 1) / (16 * NQ) - (int)(blockIdx.x / p.splits / p.n_kv)) * (16 * NQ);
     const int row1 = row0 + 16 * NQ < rows ? row0 + 16 * NQ : rows;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Kv8Wave<D, NQ> w;
@@ -625,15 +625,15 @@ tlhip_status attn_d(hipStream_t s, Kv8Attn p, const Kv8Plan& pl) {
     const int rows = p.S * p.group;
     if (pl.splits == 0) {
         const int wg = (rows + 64 * pl.nq - 1) / (64 * pl.nq) * p.n_kv;
-        if constexpr (D <= 128)
-            if (pl.nq == 2) kv8_attn_rows_kernel<D, 2><<<wg, 256, 0, s>>>(p);
-        if (pl.nq == 1) kv8_attn_rows_kernel<D, 1><<<wg, 256, 0, s>>>(p);
+        if constexpr (D > 64) kv8_attn_rows_kernel<D, D == 256 ? 1 : 2><<<wg, 256, 0, s>>>(p);
         return TLHIP_OK;
     }
     p.splits = pl.splits;
     const int wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * p.n_kv * pl.splits;
     if constexpr (D <= 128)
         if (pl.nq == 2) kv8_attn_keys_kernel<D, 2><<<wg, 256, 0, s>>>(p);
+    if constexpr (D <= 64)
+        if (pl.nq == 4) kv8_attn_keys_kernel<D, 4><<<wg, 256, 0, s>>>(p);
     if (pl.nq == 1) kv8_attn_keys_kernel<D, 1><<<wg, 256, 0, s>>>(p);
     if (pl.splits > 1) kv8_join_kernel<D><<<rows * p.n_kv, 256, 0, s>>>(p);
     return TLHIP_OK;
@@ -675,25 +675,28 @@ tlhip_status launch_kv8_read(hipStream_t s, const Kv8Read& p) {
     return TLHIP_OK;
 }
 
-// How a call is spread over the device.  A wave takes two columns of 16 rows
-// when there are more rows than one has (a tile is unpacked once for both:
-// 2048 rows of 32 / 4 heads of 64 37.6 us against 48 with one and 65 with
-// four; 700 after 5300 93 against 167), one at head dim 256, whose sums fill
-// the registers.  With 2048 or more such columns a wave walks all keys of its
-// own (splits = 0: 2048 rows of 32 / 8 heads of 128 61 us against 72), with
-// fewer the four waves of a workgroup share the keys (1024 rows of 32 heads of
-// 80: 21 us against 28); and below 512 workgroups the keys are cut into
-// splits, up to two workgroups a CU, four tiles each at least.  (Up to four a
-// CU: 300 rows after 3000, 32 / 4 heads of 64, 35 us against 25, one row after
-// 20000, 32 / 8 of 128, 17.4 against 13.9; up to one: 12.2 there, but 65000
-// keys of 32 heads of 80 67.7 against 64.5.)
+// How a call is spread over the device (figures: calls on three caches in
+// turn, from Python).  A wave takes two columns of 16 rows
+// when there are more rows than one has (a tile is unpacked once for both: 700
+// rows after 5300, 32 / 8 heads of 128, 104 us against 167 with one), four up
+// to head dim 64 if they still make 1024 workgroups (2048 rows of 32 / 4 heads
+// of 64 36.5 us against 41.3 with two, after 4000 116 against 137; 1024 rows,
+// 512 workgroups, 16.1 against 14.6), one at head dim 256, whose sums fill the
+// registers.  From 2048 pairs of columns on a wave walks all keys of its own,
+// and the waves of a workgroup meet in its cache (splits = 0: 2048 rows of 32 /
+// 8 heads of 128 62 us against 72); with fewer, or four columns, the four waves
+// share the keys (1024 rows of 32 heads of 80: 20 us against 28); and below
+// 512 workgroups the keys are cut into splits, up to two workgroups a CU, four
+// tiles each at least.  (Up to four a CU: 300 rows after 3000, 32 / 4 heads of
+// 64, 35 us against 25, one row after 20000, 32 / 8 of 128, 17.4 against 13.9;
+// up to one: 12.2 there, but 65000 keys of 32 heads of 80 67.7 against 64.5.)
 Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     Kv8Plan pl;
     const int64_t rows = (int64_t)S * group;
     const int tiles = (len + 31) / 32;
-    pl.nq = rows <= 16 || D > 128 ? 1 : 2;
+    pl.nq = rows <= 16 || D > 128 ? 1 : D <= 64 && rows * n_kv >= 1024 * 64 ? 4 : 2;
     const int64_t wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * n_kv;
-    if (wg >= 2048) return pl;
+    if (pl.nq <= 2 && wg >= 2048) return pl;
     int64_t splits = 512 / wg;
     if (splits < 1) splits = 1;
     if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;

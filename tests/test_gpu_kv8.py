@@ -207,21 +207,21 @@ def test_rows_before_a_bad_block_in_one_tile_of_rows(dev, S, past):
         check(got[:first], q[:first], kv[0][:32], kv[1][:32], 0.125, "before") if first == 32 - past else None
 
 
-@pytest.mark.parametrize("S,past,H", [(1, 0, 4), (1, 190, 4), (60, 140, 4), (100, 140, 256), (140, 100, 512)])
+@pytest.mark.parametrize("S,past,H,D", [(1, 0, 4, 64), (1, 190, 4, 64), (60, 140, 4, 64), (100, 140, 256, 64), (140, 100, 512, 64), (140, 100, 512, 80)])
 @pytest.mark.parametrize("power", [20, 27, 40])
-def test_values_of_blocks_far_apart(dev, S, past, H, power):
+def test_values_of_blocks_far_apart(dev, S, past, H, D, power):
     """Blocks of V whose sizes lie up to 2^40 apart (zeros among them), seen with weights alike: each
     weight counts with its full precision in the sum, and the large values with theirs in the result."""
     n = S + past
-    k, v = rows(12, n, 2, 64)
+    k, v = rows(12, n, 2, D)
     size = np.array([8, 8 - power, 8 - power, 8 - power, None, 8 - power // 2, -14], dtype=object)
     for b in range((n + 31) // 32):
         e = size[b % 7]
         blk = v[32 * b:32 * b + 32].astype(np.float64)
         blk = blk / np.abs(blk).max(axis=(0, 2), keepdims=True)
         v[32 * b:32 * b + 32] = 0 if e is None else np.maximum(np.abs(blk) * 2.0 ** max(e, -24), 2.0 ** -24) * np.sign(blk)
-    q = (np.random.default_rng(n).standard_normal((S, H, 64)) / 4).astype(np.float16)
-    c = KVCache(dev, 1, n, 2, 64, Q8_0)
+    q = (np.random.default_rng(n).standard_normal((S, H, D)) / 4).astype(np.float16)
+    c = KVCache(dev, 1, n, 2, D, Q8_0)
     c.set(0, dev.tensor(k), dev.tensor(v))
     got = c.attention(dev.tensor(q), 0, 0.125).numpy()
     kk, vv = held(k), held(v)
@@ -232,7 +232,7 @@ def test_values_of_blocks_far_apart(dev, S, past, H, power):
         assert p[p > 0].min() > 2.0 ** -12   # all weights are of normal size: attend()'s term for the smaller ones falls away
         p /= p.sum(1, keepdims=True)
         absum = p @ np.abs(vv[:, h // (H // 2)])
-        dsc = 70 * 2.0 ** -24 * (np.abs(q[:, h].astype(np.float64)) @ np.abs(kk[:, h // (H // 2)]).T) * 0.125 + 2.0 ** -22 * (np.abs(np.where(sc > -np.inf, sc, 0)) + 40)
+        dsc = (D + 6) * 2.0 ** -24 * (np.abs(q[:, h].astype(np.float64)) @ np.abs(kk[:, h // (H // 2)]).T) * 0.125 + 2.0 ** -22 * (np.abs(np.where(sc > -np.inf, sc, 0)) + 40)
         t = 2.0 ** -11 * (np.abs(ref[:, h]) + 2 * absum) + (2 * dsc.max(1, keepdims=True) + n * 2.0 ** -24) * absum + 2.0 ** -25
         assert (np.abs(got[:, h] - ref[:, h]) <= t).all(), float((np.abs(got[:, h] - ref[:, h]) / t).max())
 
