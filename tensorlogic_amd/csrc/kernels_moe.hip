@@ -32,6 +32,7 @@
 // hi + lo, with the power of two that puts the token's largest |h| just below
 // 2^15: 22 bits of every h, and none lost to the range of f16.
 #include <cmath>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "internal.hpp"
@@ -77,23 +78,45 @@ __global__ __launch_bounds__(1024) void moe_router_kernel(MoeArgs a) {
     const int P = a.E <= 2 ? 8 : a.E <= 4 ? 4 : a.E <= 8 ? 2 : 1;
     const uint16_t* x = a.x + (size_t)m * a.K;
     const int pieces = a.K / 8, share = (pieces + P - 1) / P;
-    for (int task = wave; task < a.E * P; task += 16) {
-        const int e = task / P, k0 = (task % P) * share, k1 = k0 + share < pieces ? k0 + share : pieces;
-        const uint16_t* r = a.router + (size_t)e * a.K;
-        float s = 0.0f;
-#pragma unroll 4
-        for (int k = k0 + lane; k < k1; k += 64) {
-            const u4 xv = *(const u4*)(x + 8 * k), rv = *(const u4*)(r + 8 * k);
+    // U tasks t0, t0 + 16, ... at once, their loads in flight together (E = 32,
+    // K = 1024: 4.0 us with two, 5.0 with one after the other)
+    auto tasks = [&](auto at_once, int t0) {
+        constexpr int U = decltype(at_once)::value;
+        const int k0 = t0 % P * share, have = share < pieces - k0 ? share : pieces - k0;   // (U > 1: P = 1)
+        const uint16_t* r[U];
+        float s[U];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const h2 p = as_h2(xv[i]), q = as_h2(rv[i]);
-                s = fmaf((float)p[0], (float)q[0], s);
-                s = fmaf((float)p[1], (float)q[1], s);
-            }
+        for (int u = 0; u < U; u++) {
+            r[u] = a.router + (size_t)((t0 + 16 * u) / P) * a.K + 8 * k0;
+            s[u] = 0.0f;
         }
-        s = wave_sum<64>(s);
-        if (lane == 0) (P == 1 ? lg : part)[task] = s;
+#pragma unroll 4 / U
+        for (int k = lane; k < have; k += 64) {
+            const u4 xv = *(const u4*)(x + 8 * (k0 + k));
+            u4 rv[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) rv[u] = *(const u4*)(r[u] + 8 * k);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const h2 p = as_h2(xv[i]), q = as_h2(rv[u][i]);
+                    s[u] = fmaf((float)p[0], (float)q[0], s[u]);
+                    s[u] = fmaf((float)p[1], (float)q[1], s[u]);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            s[u] = wave_sum<64>(s[u]);
+            if (lane == 0) (P == 1 ? lg : part)[t0 + 16 * u] = s[u];
+        }
+    };
+    int t0 = wave;
+    if (P == 1) {
+        for (; t0 + 48 < a.E; t0 += 64) tasks(std::integral_constant<int, 4>{}, t0);
+        for (; t0 + 16 < a.E; t0 += 32) tasks(std::integral_constant<int, 2>{}, t0);
     }
+    for (; t0 < a.E * P; t0 += 16) tasks(std::integral_constant<int, 1>{}, t0);
     __syncthreads();
     if (P > 1 && (int)threadIdx.x < a.E) {
         float s = 0.0f;
