@@ -690,6 +690,9 @@ tlhip_status launch_kv8_read(hipStream_t s, const Kv8Read& p) {
 // tiles each at least.  (Up to four a CU: 300 rows after 3000, 32 / 4 heads of
 // 64, 35 us against 25, one row after 20000, 32 / 8 of 128, 17.4 against 13.9;
 // up to one: 12.2 there, but 65000 keys of 32 heads of 80 67.7 against 64.5.)
+// Up to 1024 keys (512 for two columns or head dim 256) are not split: a step
+// at 400 keys, 32 / 4 heads of 64, 5.7 us against 8.7 with the join's launch, at
+// 900 6.4 against 10.1; 1900 of 32 heads of 80 would take 11.6 against 8.7.
 Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     Kv8Plan pl;
     const int64_t rows = (int64_t)S * group;
@@ -697,7 +700,7 @@ Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     pl.nq = rows <= 16 || D > 128 ? 1 : D <= 64 && rows * n_kv >= 1024 * 64 ? 4 : 2;
     const int64_t wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * n_kv;
     if (pl.nq <= 2 && wg >= 2048) return pl;
-    int64_t splits = 512 / wg;
+    int64_t splits = tiles * pl.nq * (D > 128 ? 2 : 1) <= 32 ? 1 : 512 / wg;
     if (splits < 1) splits = 1;
     if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
     pl.splits = (int)splits;
