@@ -789,10 +789,12 @@ static_assert((64 << 10) + (32 << 10) + 64 * (kMoeMaxRow / 32) <= kLdsDynamic, "
 static_assert(kDownColumnBytes + (64 << 10) <= kLdsDynamic && (32 << 10) + (64 << 10) <= kLdsDynamic, "f16 rows fit");
 
 // Up to 16 (down: 8) tokens, no expert has more columns than one B operand holds.
+int gate_up_columns(const MoeArgs& a) { return a.M < 32 ? a.M : 32; }
+int down_columns(const MoeArgs& a) { return a.M < 16 ? 2 * a.M : 32; }
 template <int WT, int KS>
 void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
     const unsigned grid = slots * ((a.I / 16 + kWaves / KS - 1) / (kWaves / KS));
-    const Layout at = layout<WT, 2, KS, kWaves>(a.K / 32, a.M < 32 ? a.M : 32);
+    const Layout at = layout<WT, 2, KS, kWaves>(a.K / 32, gate_up_columns(a));
     if (a.M == 1) moe_gate_up_kernel<WT, KS, 1, true><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     else if (a.M <= 16) moe_gate_up_kernel<WT, KS, 1, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
     else moe_gate_up_kernel<WT, KS, 2, false><<<grid, kWaves * 64, at.bytes, s>>>(a, at);
@@ -800,23 +802,33 @@ void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
 template <int WT, int KS, int NW>
 void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
     const unsigned grid = slots * ((a.K / 16 + NW / KS - 1) / (NW / KS));
-    const Layout at = layout<WT, 1, KS, NW>(a.I / 32, a.M < 16 ? 2 * a.M : 32);
+    const Layout at = layout<WT, 1, KS, NW>(a.I / 32, down_columns(a));
     if (a.M <= 8) moe_down_kernel<WT, KS, 1, NW><<<grid, NW * 64, at.bytes, s>>>(a, at);
     else moe_down_kernel<WT, KS, 2, NW><<<grid, NW * 64, at.bytes, s>>>(a, at);
     moe_sum_kernel<<<(a.M * (a.K / 4) + 255) / 256, 256, 0, s>>>(a);
 }
+// How often a CU fills up with workgroups until all have run.
+template <int WT, int NR, int KS, int NW>
+int64_t turns(int64_t tiles, int nb, int columns) {
+    const int fit = (160 << 10) / (layout<WT, NR, KS, NW>(nb, columns).bytes + (int)sizeof(MoeShared));
+    return (tiles * KS / NW + 256 * fit - 1) / (256 * fit);
+}
 // Waves that share out the k of a tile of 16 rows: as few as leave two
 // workgroups of four waves for every CU (the more tiles a workgroup has, the
-// fewer times the columns are staged), and no fewer than LDS has room for.
+// fewer times the columns are staged), and no fewer than LDS has room for; for
+// few tiles two, if a CU then fills up with workgroups less often (28 tokens of
+// four Q4_0 experts 2656 x 1056, all chosen: 49 us against 75; 12 of six f16
+// ones 2048 x 1024, two each: 26 against 33).
 template <int WT, int NR, int NW>
-int waves_of_tile(int64_t tiles, int nb) {
-    if (tiles >= 2048 && layout<WT, NR, 1, NW>(nb, 32).bytes <= kLdsDynamic) return 1;
-    if (tiles >= 1024 && layout<WT, NR, 2, NW>(nb, 32).bytes <= kLdsDynamic) return 2;
+int waves_of_tile(int64_t tiles, int nb, int columns) {
+    if (tiles >= 2048 && layout<WT, NR, 1, NW>(nb, columns).bytes <= kLdsDynamic) return 1;
+    const bool two = layout<WT, NR, 2, NW>(nb, columns).bytes <= kLdsDynamic;
+    if (two && (tiles >= 1024 || turns<WT, NR, 2, NW>(tiles, nb, columns) < turns<WT, NR, 4, NW>(tiles, nb, columns))) return 2;
     return 4;
 }
 template <int WT>
 void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    switch (waves_of_tile<WT, 2, kWaves>((int64_t)slots * (a.I / 16), a.K / 32)) {
+    switch (waves_of_tile<WT, 2, kWaves>((int64_t)slots * (a.I / 16), a.K / 32, gate_up_columns(a))) {
         case 1: return gate_up<WT, 1>(s, a, slots);
         case 2: return gate_up<WT, 2>(s, a, slots);
         default: return gate_up<WT, 4>(s, a, slots);
@@ -824,7 +836,7 @@ void gate_up(hipStream_t s, const MoeArgs& a, unsigned slots) {
 }
 template <int WT, int NW>
 void down_waves(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    switch (waves_of_tile<WT, 1, NW>((int64_t)slots * (a.K / 16), a.I / 32)) {
+    switch (waves_of_tile<WT, 1, NW>((int64_t)slots * (a.K / 16), a.I / 32, down_columns(a))) {
         case 1: return down<WT, 1, NW>(s, a, slots);
         case 2: return down<WT, 2, NW>(s, a, slots);
         default: return down<WT, 4, NW>(s, a, slots);
