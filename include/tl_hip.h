@@ -303,7 +303,8 @@ tlhip_status tlhip_token_logprobs(tlhip_ctx ctx, tlhip_tensor logits, tlhip_tens
  * multiples of 32 up to 16384, E <= 256, top_k <= min(E, 32).  The weights
  * count as the f16 values that linear() reads them as; what lies between x
  * and y is not rounded to f16.  y may be x.  Any M; the weights an expert's
- * tokens need are read once for up to 256 tokens.                          */
+ * tokens need are read once for up to 256 tokens (down's once a token where
+ * that is faster for a few).                                               */
 tlhip_status tlhip_moe(tlhip_ctx ctx, tlhip_tensor x, tlhip_tensor router, tlhip_tensor gate, tlhip_tensor up,
                        tlhip_tensor down, int top_k, int normalize, tlhip_tensor y);
 

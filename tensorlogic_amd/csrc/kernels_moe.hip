@@ -13,9 +13,9 @@
 // 41, 4.7 TB/s; down 26; router and sum 4 each).
 //
 // Four launches: the router (a workgroup per token); gate and up; down; the
-// sum over a token's experts (three for one token, whose down sums them
-// itself).  What bounds the middle two is reading the weights of the experts
-// that some token chose, so each is read once: a wave takes 16 rows of one
+// sum over a token's experts (three for one token and for a few, whose down
+// sums them itself).  What bounds the middle two is reading the weights of the
+// experts that some token chose, so each is read once: a wave takes 16 rows of one
 // expert (of gate and of up both) and multiplies by all of that expert's
 // tokens on the matrix cores (v_mfma_f32_16x16x32_f16, A = 16 weight rows x 32
 // k, B = 32 k x 16 columns; unused columns cost nothing that is scarce).
@@ -665,11 +665,12 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
     *(uint64_t*)y = (uint64_t)f2h(s[0]) | (uint64_t)f2h(s[1]) << 16 | (uint64_t)f2h(s[2]) << 32 | (uint64_t)f2h(s[3]) << 48;
 }
 
-// Down for a single token: all its experts in one workgroup per 16 rows, so
-// that no sum is left over.  Sixteen waves share out the (expert, slot) pairs;
+// Down token by token: all its experts in one workgroup per 16 rows, so that
+// no sum is left over.  Sixteen waves share out the (expert, slot) pairs;
 // the columns are hi and lo of h under one power of two, all of them in LDS at
 // once: blocks of expert t from t * per slots on.
 constexpr int kOneWaves = 16, kOneRing = 2, kOnePieces = 2;
+constexpr int kOneStatic = kOneWaves * 33 * 4;   // its LDS beside the dynamic part
 template <int WT>
 __host__ __device__ inline Layout layout_one(int nb, int top) {
     const int per = (nb + Slot<WT>::BLOCKS - 1) / Slot<WT>::BLOCKS;
@@ -691,7 +692,8 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
     const uint8_t* ring = lds + at.ring_at + wave * (kOneRing * S::BYTES);
     const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(ring));
     const uint8_t* scales = lds + at.scales_at;
-    const int ids = a.ids[lane < a.top ? lane : 0];
+    const size_t pair0 = (size_t)blockIdx.y * a.top;   // of the token
+    const int ids = a.ids[pair0 + (lane < a.top ? lane : 0)];
     auto copy = [&](int n, int k) {
         const int t = n / per, e = __builtin_amdgcn_readlane(ids, t);
         Rows<WT>(a.down, (size_t)e * a.K + n0, nb).copy(n - t * per, ring_lds + k * S::BYTES);
@@ -705,7 +707,7 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
             const int i = i0 + k * kOneWaves * 64, s = i & 3, t = (i >> 2) / (per * S::BLOCKS), b = (i >> 2) - t * (per * S::BLOCKS);
             p[k] = q[k] = f4{0, 0, 0, 0};
             if (i < slots * S::BLOCKS * 4 && b < nb) {
-                const float* h = a.h + (size_t)t * a.I + b * 32;
+                const float* h = a.h + (pair0 + t) * a.I + b * 32;
                 p[k] = *(const f4*)(h + run0<WT>(s));
                 q[k] = *(const f4*)(h + run1<WT>(s));
             }
@@ -713,7 +715,7 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
     };
     fetch(threadIdx.x);
     float m = 0.0f;
-    for (int i = threadIdx.x; i < a.top * (a.I / 16); i += kOneWaves * 64) m = fmaxf(m, a.hmax[i]);
+    for (int i = threadIdx.x; i < a.top * (a.I / 16); i += kOneWaves * 64) m = fmaxf(m, a.hmax[pair0 * (a.I / 16) + i]);
     m = wave_max(m);
     if (lane == 0) most[wave] = m;
     if constexpr (WT != TLHIP_F16) {
@@ -776,7 +778,7 @@ __global__ __launch_bounds__(kOneWaves * 64) void moe_down_one_kernel(MoeArgs a,
     if (threadIdx.x < 16) {
         float s = 0.0f;
         for (int w = 0; w < kOneWaves; w++) s += red[w][0][threadIdx.x] + red[w][1][threadIdx.x];
-        a.y[n0 + threadIdx.x] = f2h(s / scale);
+        a.y[(size_t)blockIdx.y * a.K + n0 + threadIdx.x] = f2h(s / scale);
     }
 }
 
@@ -844,12 +846,15 @@ void down_waves(hipStream_t s, const MoeArgs& a, unsigned slots) {
 }
 template <int WT>
 void down(hipStream_t s, const MoeArgs& a, unsigned slots) {
-    if (a.M == 1) {
-        const Layout at = layout_one<WT>(a.I / 32, a.top);
-        if (at.bytes <= kLdsDynamic) {
-            moe_down_one_kernel<WT><<<a.K / 16, kOneWaves * 64, at.bytes, s>>>(a, at);
-            return;
-        }
+    // A token's workgroups read its experts' weights whether or not another's
+    // do, but no sum is left to launch: taken for one token, and for a few whose
+    // workgroups all run at once (two to eight: 4 us less; four of K = 4096,
+    // 1024 workgroups of which 256 fit, would take 40 us against 37).
+    const Layout at = layout_one<WT>(a.I / 32, a.top);
+    const int fit = at.bytes + kOneStatic <= 80 << 10 ? 2 : 1;
+    if (at.bytes + kOneStatic <= 160 << 10 && (a.M == 1 || a.M * (a.K / 16) <= 256 * fit)) {
+        moe_down_one_kernel<WT><<<dim3(a.K / 16, a.M), kOneWaves * 64, at.bytes, s>>>(a, at);
+        return;
     }
     if (a.M * a.top >= 2 * a.E) down_waves<WT, kDownWaves>(s, a, slots);
     else down_waves<WT, kWaves>(s, a, slots);

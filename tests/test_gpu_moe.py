@@ -92,6 +92,13 @@ def test_against_64_bits(dev, gu, dn, M, E, K, I, top):
     run(dev, 1, M, E, K, I, top, (M + E) % 2 == 0, gu, dn)
 
 
+@pytest.mark.parametrize("gu,dn", [(F16, F16), (Q4_0, Q8_0), (Q8_0, Q4_0)])
+@pytest.mark.parametrize("M,E,K,I,top", [(7, 4, 2048, 96, 2), (8, 3, 1088, 224, 3), (9, 4, 2048, 64, 3), (17, 3, 1024, 160, 1),
+                                         (24, 64, 512, 64, 6), (33, 8, 352, 224, 2), (40, 5, 416, 96, 2), (130, 2, 160, 96, 1)])
+def test_more_workgroups_than_run_at_once(dev, gu, dn, M, E, K, I, top):
+    run(dev, 6, M, E, K, I, top, M % 2 == 0, gu, dn)
+
+
 @pytest.mark.parametrize("M,E,K,I,top,gu", [(1, 8, 2048, 5632, 2, Q4_0), (13, 8, 1024, 1408, 2, Q8_0), (70, 16, 512, 320, 4, Q4_0), (2, 256, 64, 64, 32, F16),
                                             (5, 2, 4096, 32, 2, Q8_0), (4, 2, 32, 4128, 1, Q4_0), (300, 4, 96, 64, 2, Q8_0), (600, 2, 32, 32, 1, F16)])
 def test_larger(dev, M, E, K, I, top, gu):
