@@ -129,6 +129,19 @@ struct Batch {
         const int i = index(j);
         return i >= lo && i >= place(j / W) && i < hi;
     }
+    // A set of elements, the first at the highest of E bits.
+    static constexpr uint32_t ALL = 0xFFFFFFFFu >> (32 - E);
+    static __device__ __forceinline__ uint32_t bit(int j) { return 1u << (E - 1 - j); }
+    static __device__ __forceinline__ int first(uint32_t set) { return __builtin_clz(set & ALL) - (32 - E); }
+    // The elements less than y (above: greater): the differences' signs, shifted
+    // in.  (A comparison's mask would take a move and two waits each.)  NaN: any.
+    __device__ __forceinline__ uint32_t below(float y, bool above) const {
+        if (y == 0.0f) y = above ? 0.0f : -0.0f;   // (either zero minus it is +0)
+        uint32_t set = 0;
+#pragma unroll
+        for (int j = 0; j < E; j++) set = __builtin_amdgcn_alignbit(set, __float_as_uint(above ? y - (*this)[j] : (*this)[j] - y), 31);
+        return set;
+    }
     __device__ __forceinline__ void set(int j, float x) {
         if constexpr (F32) f[j] = x;
         else h[j / 8][j % 8] = (h16)x;
@@ -289,8 +302,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
                 // the first element that is m (an -inf in place of another is none)
                 int first = -1;
                 if (m > -INFINITY) {
-#pragma unroll
-                    for (int j = E - 1; j >= 0; j--) first = x[j] == m ? j : first;
+                    const uint32_t less = x.below(m, false);
+                    first = less != Batch<F32, E>::ALL ? Batch<F32, E>::first(~less) : -1;
                 } else {
                     for (int j = E - 1; j >= 0; j--) first = x[j] == m && x.mine(j) ? j : first;
                 }
@@ -300,21 +313,20 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
             const float least = tau ? key_value(tau) : -INFINITY;
             if (m >= least) {
                 // the places of the batch's keys from tau up go to the list
-                uint32_t hit = 0, even = 0;
-#pragma unroll
-                for (int j = 0; j < E; j++) {
-                    hit |= x[j] > least ? 1u << j : 0;
-                    even |= x[j] == least ? 1u << j : 0;
-                }
+                // (-inf has no differences: the lowest finite value stands in)
+                const bool any = least == -INFINITY;
+                const float l = any ? -3.4028234663852886e38f : least;
+                const uint32_t less = x.below(l, false), more = x.below(l, true), same = Batch<F32, E>::ALL & ~(less | more);
+                uint32_t hit = any ? more | same : more, even = any ? less : same;
                 const int last = tau ? key_index(tau) - begin - at0 : Batch<F32, E>::SIZE;
-                for (; even; even &= even - 1) {
-                    const int j = __builtin_ctz(even);
-                    if (x.mine(j) && x.index(j) <= last) hit |= 1u << j;
+                for (; even; even ^= Batch<F32, E>::bit(Batch<F32, E>::first(even))) {
+                    const int j = Batch<F32, E>::first(even);
+                    if (x.mine(j) && x.index(j) <= last) hit |= Batch<F32, E>::bit(j);
                 }
                 if (hit) {
                     int slot = atomicAdd(&sh.count, __builtin_popcount(hit));
-                    for (; hit; hit &= hit - 1, slot++)
-                        if (slot < kList) sh.list[slot] = at0 + x.index(__builtin_ctz(hit));
+                    for (; hit; hit ^= Batch<F32, E>::bit(Batch<F32, E>::first(hit)), slot++)
+                        if (slot < kList) sh.list[slot] = at0 + x.index(Batch<F32, E>::first(hit));
                 }
             }
             if (nb && !(nb & (nb + 1)) && b + Batch<F32, E>::SIZE < count) tau = bound(best, a.n_top, sh);
