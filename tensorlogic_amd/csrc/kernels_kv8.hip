@@ -623,11 +623,12 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attn p) {
 template <int D>
 tlhip_status attn_d(hipStream_t s, Kv8Attn p, const Kv8Plan& pl) {
     const int rows = p.S * p.group;
-    if (pl.splits == 0) {
-        const int wg = (rows + 64 * pl.nq - 1) / (64 * pl.nq) * p.n_kv;
-        if constexpr (D > 64) kv8_attn_rows_kernel<D, D == 256 ? 1 : 2><<<wg, 256, 0, s>>>(p);
-        return TLHIP_OK;
-    }
+    if constexpr (D > 64)
+        if (pl.splits == 0) {
+            constexpr int NQ = D == 256 ? 1 : 2;
+            kv8_attn_rows_kernel<D, NQ><<<(rows + 64 * NQ - 1) / (64 * NQ) * p.n_kv, 256, 0, s>>>(p);
+            return TLHIP_OK;
+        }
     p.splits = pl.splits;
     const int wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * p.n_kv * pl.splits;
     if constexpr (D <= 128)
@@ -682,10 +683,11 @@ tlhip_status launch_kv8_read(hipStream_t s, const Kv8Read& p) {
 // to head dim 64 if they still make 1024 workgroups (2048 rows of 32 / 4 heads
 // of 64 36.5 us against 41.3 with two, after 4000 116 against 137; 1024 rows,
 // 512 workgroups, 16.1 against 14.6), one at head dim 256, whose sums fill the
-// registers.  From 2048 pairs of columns on a wave walks all keys of its own,
-// and the waves of a workgroup meet in its cache (splits = 0: 2048 rows of 32 /
-// 8 heads of 128 62 us against 72); with fewer, or four columns, the four waves
-// share the keys (1024 rows of 32 heads of 80: 20 us against 28); and below
+// registers.  From 2048 workgroups of shared keys on, past head dim 64, a wave
+// walks all keys of its own instead, and the waves of a workgroup meet in its
+// CU's cache (splits = 0: 2048 rows of 32 / 8 heads of 128 62 us against 72);
+// else the four waves share them (1024 rows of 32 heads of 80: 20 us against
+// 28; up to head dim 64 the two measure the same, 41 us); and below
 // 512 workgroups the keys are cut into splits, up to two workgroups a CU, four
 // tiles each at least.  (Up to four a CU: 300 rows after 3000, 32 / 4 heads of
 // 64, 35 us against 25, one row after 20000, 32 / 8 of 128, 17.4 against 13.9;
@@ -699,7 +701,7 @@ Kv8Plan kv8_plan(int S, int group, int n_kv, int D, int len) {
     const int tiles = (len + 31) / 32;
     pl.nq = rows <= 16 || D > 128 ? 1 : D <= 64 && rows * n_kv >= 1024 * 64 ? 4 : 2;
     const int64_t wg = (rows + 16 * pl.nq - 1) / (16 * pl.nq) * n_kv;
-    if (pl.nq <= 2 && wg >= 2048) return pl;
+    if (D > 64 && wg >= 2048) return pl;
     int64_t splits = tiles * pl.nq * (D > 128 ? 2 : 1) <= 32 ? 1 : 512 / wg;
     if (splits < 1) splits = 1;
     if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;

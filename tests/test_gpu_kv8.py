@@ -141,7 +141,10 @@ def test_attention(dev, H, kv, D, S, past):
 @pytest.mark.parametrize("H,kv,D,S,past", [(32, 4, 64, 300, 0), (32, 32, 80, 40, 100), (16, 1, 64, 1, 5000), (8, 8, 128, 1, 4111),
                                            (40, 1, 64, 1, 500), (128, 2, 32, 3, 100), (4, 1, 64, 700, 1300), (64, 64, 64, 17, 333),
                                            # enough rows for a wave to take all keys of its own
-                                           (256, 8, 32, 260, 37), (256, 8, 64, 260, 300), (512, 4, 80, 135, 1), (256, 16, 128, 260, 0), (256, 1, 256, 131, 20)])
+                                           (256, 8, 32, 260, 37), (256, 8, 64, 260, 300), (512, 4, 80, 135, 1), (256, 16, 128, 260, 0), (256, 1, 256, 131, 20),
+                                           # few rows of many heads: as many workgroups
+                                           (1024, 1024, 32, 40, 5), (1024, 1024, 64, 33, 0), (1024, 1024, 64, 17, 50), (1024, 1024, 80, 33, 2),
+                                           (2048, 1024, 96, 20, 0), (1024, 1024, 128, 33, 40), (1024, 512, 256, 40, 3), (1024, 1024, 64, 1, 300)])
 def test_attention_larger(dev, H, kv, D, S, past):
     test_attention(dev, H, kv, D, S, past)
 
